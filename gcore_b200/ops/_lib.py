@@ -7,6 +7,7 @@ silently degrades to eager PyTorch.  ``GCORE_B200_FORCE_EAGER=1`` selects the Py
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 from pathlib import Path
@@ -105,6 +106,21 @@ def stream_ptr():
     """The current stream of the current device.  ``torch.cuda.current_stream`` looks the device up through the environment
     and builds a stream object on every call; without that a served pass of 306 launches submits 1.3 ms sooner."""
     return c_void_p(torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice()))
+
+
+def on_device(t: torch.Tensor):
+    """Context in which ``t``'s device is the current one, so that a launch goes to a stream of that device."""
+    if t.get_device() == torch._C._cuda_getDevice():
+        return _HERE_ALREADY
+    return torch.cuda.device(t.device)
+
+
+_HERE_ALREADY = contextlib.nullcontext()
+
+
+def packed16(t: torch.Tensor) -> torch.Tensor:
+    """``t`` itself where it is contiguous and starts on a 16-byte boundary, else a copy that is and does."""
+    return t if t.is_contiguous() and t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
 
 
 def check(rc: int, what: str):
@@ -214,6 +230,10 @@ def _declare_kernels(lib: ctypes.CDLL):
     d("gk_sample_filtered", [P, I, L, I, F, I, F, F, I, P, P, P, P, P, I, P])
     d("gk_rope_copy", [P, P, P, I, I, I, I, I, F, I, I, P])
     d("gk_dequant_128x128", [P, P, P, L, I, P])
+    d("gk_norm_quant", [P, P, P, P, P, P, I, I, F, I, I, P])
+    d("gk_rows_quant", [P, P, P, L, I, I, I, I, P])
+    d("gk_fp4_dequant", [P, P, P, L, I, P])
+    d("gk_mxfp8_dequant", [P, P, P, L, I, P])
     d("gk_mla_expand", [P, P, P, P, I, I, I, I, I, P])
     d("gk_mla_expand_bwd", [P, P, P, P, I, I, I, I, I, P])
     d("gk_latent_append", [P, L, P, P, P, P, I, I, I, F, F, I, P])

@@ -1,0 +1,235 @@
+// Rows that end in e4m3: residual addition + RMSNorm, SwiGLU and plain rows, each quantised in the pass that computes it.
+//
+//   SC32 = false  one fp32 scale per 128 values, amax / 448 (what gemm_fp8.cu reads)
+//   SC32 = true   one power of two per 32 values as its biased exponent (e8m0, what gemm_fp4.cu reads): the smallest that keeps
+//                 the group within 448.  A NaN or an infinity in the group makes the exponent 255, which is NaN.
+//
+// Values stay in 32 bits from the input to the one rounding at the end.  AS16 rounds them to bf16 first, so that the codes and
+// scales are those of the unfused kernels (norm or activation to bf16, then the quantiser) bit for bit: the order of every sum
+// is rmsnorm_fwd_kernel's (elementwise.cu).
+//
+// Bound by memory: a norm reads 4 and writes 3 bytes a value with its residual, the activation reads 4 and writes 1; the chains
+// they replace write and read the bf16 value in between (4 bytes more) and launch twice.
+#include "host_utils.h"
+#include <cuda_bf16.h>
+#include <cuda_fp8.h>
+#include <type_traits>
+
+namespace gqr {
+using namespace gk;
+
+struct alignas(16) Row8 { __nv_bfloat162 v[4]; };
+
+__device__ __forceinline__ void unpack(const Row8& a, float (&f)[8]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 t = __bfloat1622float2(a.v[i]);
+    f[2 * i] = t.x;
+    f[2 * i + 1] = t.y;
+  }
+}
+__device__ __forceinline__ Row8 pack(const float (&f)[8]) {
+  Row8 a;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) a.v[i] = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
+  return a;
+}
+
+__device__ __forceinline__ uint2 codes8(const float (&f)[8], float inv) {
+  uint32_t h[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    h[i] = __nv_cvt_float2_to_fp8x2(make_float2(f[2 * i] * inv, f[2 * i + 1] * inv), __NV_SATFINITE, __NV_E4M3);
+  return make_uint2(h[0] | (h[1] << 16), h[2] | (h[3] << 16));
+}
+
+// Eight values of a thread to codes; the 16 (SC32: 4) neighbouring lanes of its group hold the group's other values.  All lanes
+// of the warp call this; `unit` counts units of eight values over the whole matrix and picks the group's scale.
+template <bool SC32, bool AS16>
+__device__ __forceinline__ void quantise(float (&f)[8], bool live, long long unit, uint2* q, void* scales) {
+  if (AS16) unpack(pack(f), f);
+  if (SC32) {
+    // the comparison of bit patterns is that of sizes, with every NaN above infinity
+    uint32_t top = __float_as_uint(1e-10f);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(f[j]) & 0x7fffffffu);
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    // 448 = 1.75 * 2^8: the exponent is amax's less 8, and one more where the mantissa is above 1.75
+    const uint32_t e = top >= 0x7f800000u ? 255u : (top >> 23) - 8u + ((top & 0x7fffffu) > 0x600000u ? 1u : 0u);
+    const float inv = __uint_as_float((254u - min(e, 253u)) << 23);
+    if (live) {
+      q[unit] = codes8(f, inv);
+      if ((threadIdx.x & 3) == 0) static_cast<uint8_t*>(scales)[unit >> 2] = static_cast<uint8_t>(e);
+    }
+  } else {
+    float amax = fabsf(f[0]);
+#pragma unroll
+    for (int j = 1; j < 8; ++j) amax = fmaxf(amax, fabsf(f[j]));
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+    const float s = fmaxf(amax, 1e-10f) / 448.f;
+    const float inv = 1.f / s;
+    if (live) {
+      q[unit] = codes8(f, inv);
+      if ((threadIdx.x & 15) == 0) static_cast<float*>(scales)[unit >> 4] = s;
+    }
+  }
+}
+
+__device__ __forceinline__ float block_sum(float v, float* red) {
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  __syncthreads();
+  if (lane == 0) red[w] = v;
+  __syncthreads();
+  const int nw = (blockDim.x + 31) >> 5;
+  float t = lane < nw ? red[lane] : 0.f;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+  return t;
+}
+
+// A CTA per row, SLOTS units of eight values per thread, kept in registers between the sum and the scaling.
+template <int SLOTS, bool SC32, bool AS16>
+__global__ void __launch_bounds__(256) norm_quant_kernel(const Row8* __restrict__ x, const Row8* __restrict__ res,
+                                                         const Row8* __restrict__ w, uint2* __restrict__ q,
+                                                         void* __restrict__ scales, Row8* __restrict__ res_out, int T, int H,
+                                                         float eps) {
+  __shared__ float red[32];
+  pdl_launch_dependents();
+  const int nv = H >> 3;
+  Row8 gain[SLOTS];
+#pragma unroll
+  for (int s = 0; s < SLOTS; ++s) {
+    const int i = threadIdx.x + s * 256;
+    if (i < nv) gain[s] = w[i];
+  }
+  pdl_wait();
+  for (int row = blockIdx.x; row < T; row += gridDim.x) {
+    const long long at = static_cast<long long>(row) * nv;
+    Row8 v[SLOTS], r[SLOTS];
+#pragma unroll
+    for (int s = 0; s < SLOTS; ++s) {
+      const int i = threadIdx.x + s * 256;
+      if (i < nv) {
+        v[s] = x[at + i];
+        if (res) r[s] = res[at + i];
+      }
+    }
+    float ss = 0.f;
+#pragma unroll
+    for (int s = 0; s < SLOTS; ++s) {
+      const int i = threadIdx.x + s * 256;
+      if (i < nv) {
+        float f[8];
+        unpack(v[s], f);
+        if (res) {
+          float g[8];
+          unpack(r[s], g);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) f[j] += g[j];
+          v[s] = pack(f);
+          res_out[at + i] = v[s];
+          unpack(v[s], f);  // the norm is that of the 16-bit stream
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) ss += f[j] * f[j];
+      }
+    }
+    ss = block_sum(ss, red);
+    const float rstd = rsqrtf(ss / H + eps);
+#pragma unroll
+    for (int s = 0; s < SLOTS; ++s) {
+      const int i = threadIdx.x + s * 256;
+      float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+      if (i < nv) {
+        float g[8];
+        unpack(v[s], f);
+        unpack(gain[s], g);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) f[j] = f[j] * rstd * g[j];
+      }
+      quantise<SC32, AS16>(f, i < nv, at + i, q, scales);
+    }
+  }
+}
+
+// ACT: in = [gate | up] of 2 F values a row, silu(gate) * up; otherwise the row itself.  One unit of eight values per thread.
+template <bool ACT, bool SC32, bool AS16>
+__global__ void __launch_bounds__(256) rows_quant_kernel(const Row8* __restrict__ in, uint2* __restrict__ q,
+                                                         void* __restrict__ scales, long long units, int nv) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const long long step = static_cast<long long>(gridDim.x) * 256;
+  for (long long u0 = blockIdx.x * 256ll; u0 < units; u0 += step) {
+    const long long u = u0 + threadIdx.x;
+    const bool live = u < units;
+    float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (live) {
+      if (ACT) {
+        const long long t = u / nv, i = u - t * nv;
+        float p[8];
+        unpack(in[2 * t * nv + i], f);
+        unpack(in[(2 * t + 1) * nv + i], p);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) f[j] = f[j] / (1.f + __expf(-f[j])) * p[j];
+      } else {
+        unpack(in[u], f);
+      }
+    }
+    quantise<SC32, AS16>(f, live, u, q, scales);
+  }
+}
+
+inline bool aligned16(const void* a) { return (reinterpret_cast<uintptr_t>(a) & 15) == 0; }
+
+}  // namespace gqr
+
+using namespace gqr;
+
+// x, res (optional, with res_out) [T, H] bf16, w [H] bf16, all 16-byte aligned; q [T, H] e4m3, scales [T, H / 128] fp32 or, with
+// sc32, [T, H / 32] e8m0.  H a multiple of 128 (sc32: 32), at most 16384.
+GK_EXPORT int gk_norm_quant(const void* x, const void* res, const void* w, void* q, void* scales, void* res_out, int T, int H,
+                            float eps, int sc32, int as16, void* stream) {
+  if (T < 0 || H <= 0 || H % (sc32 ? 32 : 128) || H > 16384) return -1;
+  if (!aligned16(x) || !aligned16(res) || !aligned16(w) || !aligned16(q) || !aligned16(res_out)) return -2;
+  if (T == 0) return 0;
+  const int sms = gk::sm_count(), grid = T < sms * 8 ? T : sms * 8, nv = H / 8;
+  auto go = [&](auto kernel) {
+    gk::launch_k(kernel, dim3(grid), dim3(256), 0, static_cast<cudaStream_t>(stream), static_cast<const Row8*>(x),
+                 static_cast<const Row8*>(res), static_cast<const Row8*>(w), static_cast<uint2*>(q), scales,
+                 static_cast<Row8*>(res_out), T, H, eps);
+    return gk::launch_status();
+  };
+  auto slots = [&](auto sc, auto as) {
+    constexpr bool S = decltype(sc)::value, A = decltype(as)::value;
+    if (nv <= 256) return go(norm_quant_kernel<1, S, A>);
+    if (nv <= 512) return go(norm_quant_kernel<2, S, A>);
+    if (nv <= 1024) return go(norm_quant_kernel<4, S, A>);
+    return go(norm_quant_kernel<8, S, A>);
+  };
+  using Y = std::true_type;
+  using N = std::false_type;
+  if (sc32) return as16 ? slots(Y{}, Y{}) : slots(Y{}, N{});
+  return as16 ? slots(N{}, Y{}) : slots(N{}, N{});
+}
+
+// act: in [T, 2 F] bf16 = [gate | up]; otherwise in [T, F].  q [T, F], scales as above; 16-byte aligned.
+GK_EXPORT int gk_rows_quant(const void* in, void* q, void* scales, long long T, int F, int act, int sc32, int as16,
+                            void* stream) {
+  if (T < 0 || F <= 0 || F % (sc32 ? 32 : 128)) return -1;
+  if (!aligned16(in) || !aligned16(q)) return -2;
+  if (T == 0) return 0;
+  const int nv = F / 8;
+  const long long units = T * nv, blocks = (units + 255) / 256, most = gk::sm_count() * 32ll;
+  auto go = [&](auto kernel) {
+    gk::launch_k(kernel, dim3(static_cast<unsigned>(blocks < most ? blocks : most)), dim3(256), 0,
+                 static_cast<cudaStream_t>(stream), static_cast<const Row8*>(in), static_cast<uint2*>(q), scales, units, nv);
+    return gk::launch_status();
+  };
+  if (!act) return sc32 ? go(rows_quant_kernel<false, true, false>) : go(rows_quant_kernel<false, false, false>);
+  if (sc32) return as16 ? go(rows_quant_kernel<true, true, true>) : go(rows_quant_kernel<true, true, false>);
+  return as16 ? go(rows_quant_kernel<true, false, true>) : go(rows_quant_kernel<true, false, false>);
+}

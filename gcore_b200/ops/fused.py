@@ -326,6 +326,83 @@ def swiglu(x: torch.Tensor, n_rows: torch.Tensor = None) -> torch.Tensor:
     return swiglu_ref(x)
 
 
+# ------------------------------------------------------------------------------------------------ rows that end in e4m3
+def _e4m3_buffers(rows, width, scales, device):
+    """Codes and scales of ``[rows, width]`` values: ``fp32`` one 32-bit scale per 128, ``e8m0`` one power of two per 32."""
+    q = torch.empty(rows, width, dtype=torch.float8_e4m3fn, device=device)
+    if scales == "fp32":
+        return q, torch.empty(rows, width // 128, dtype=torch.float32, device=device)
+    return q, torch.empty(rows, width // 32, dtype=torch.float8_e8m0fnu, device=device)
+
+
+def _check_e4m3_rows(what, x, width, scales, *others):
+    if scales not in ("fp32", "e8m0"):
+        raise ValueError(f"{what}: scales must be 'fp32' or 'e8m0', got {scales!r}")
+    if width == 0 or width % (128 if scales == "fp32" else 32):
+        raise ValueError(f"{what}: a width of {width} is not a multiple of {128 if scales == 'fp32' else 32} ({scales} scales)")
+    for t in (x, *others):
+        if t is None:
+            continue
+        if t.device != x.device:
+            raise ValueError(f"{what}: tensors on {x.device} and {t.device}")
+        if t.requires_grad and torch.is_grad_enabled():
+            raise RuntimeError(f"{what} has no gradient: call it under torch.no_grad()")
+
+
+def rmsnorm_fp8(x: torch.Tensor, w: torch.Tensor, eps: float = 1e-6, residual: torch.Tensor | None = None,
+                scales: str = "fp32", as_rounded: bool = False):
+    """``rmsnorm`` whose result is quantised in the same pass: ``(q, s, x + residual)`` with ``q`` e4m3 of ``x``'s shape (without
+    ``residual`` the third value is ``x``).  ``scales="fp32"``: ``s`` has one 32-bit scale per 128 values, what
+    ``quant.gemm_fp8_blockscaled`` reads; ``"e8m0"``: one power of two per 32 values (``torch.float8_e8m0fnu``), what
+    ``quant.gemm_fp4`` reads.  The norm is rounded once, to e4m3; with ``as_rounded`` it is rounded to ``x``'s type first, so that
+    ``q`` and ``s`` are those of ``quant_act_1x128(rmsnorm(...)[0])`` bit for bit.  Inference only."""
+    from . import quant
+    H = x.shape[-1]
+    if w.shape != (H,) or (residual is not None and residual.shape != x.shape):
+        raise ValueError(f"rmsnorm_fp8: x {tuple(x.shape)}, gain {tuple(w.shape)}"
+                         + (f", residual {tuple(residual.shape)}" if residual is not None else ""))
+    _check_e4m3_rows("rmsnorm_fp8", x, H, scales, w, residual)
+    if not (x.dtype == torch.bfloat16 and w.dtype == torch.bfloat16 and (residual is None or residual.dtype == torch.bfloat16)
+            and _lib.use_native(x) and H <= 16384):
+        xs = x if residual is None else (x.float() + residual.float()).to(x.dtype)
+        xf = xs.float()
+        y = xf * torch.rsqrt(xf.pow(2).mean(-1, keepdim=True) + eps) * w.float()
+        q, s = quant.quant_rows_ref(y.to(x.dtype) if as_rounded else y, scales)
+        return q, s, xs
+    with _lib.on_device(x):
+        x2, w2 = _lib.packed16(x), _lib.packed16(w)
+        r2 = _lib.packed16(residual) if residual is not None else None
+        T = x2.numel() // H
+        q, s = _e4m3_buffers(T, H, scales, x.device)
+        out = torch.empty_like(x2) if r2 is not None else None
+        LAUNCHES["elementwise"] += 1
+        _lib.check(_lib.kernels().gk_norm_quant(_lib.ptr(x2), _lib.ptr(r2), _lib.ptr(w2), _lib.ptr(q), _lib.ptr(s),
+                                                _lib.ptr(out), T, H, float(eps), scales == "e8m0", as_rounded,
+                                                _lib.stream_ptr()), "norm_quant")
+    return q.view(x.shape), s.view(*x.shape[:-1], s.shape[1]), x if out is None else out
+
+
+def swiglu_fp8(x: torch.Tensor, scales: str = "fp32", as_rounded: bool = False):
+    """``swiglu`` whose result is quantised in the same pass: ``(q, s)`` with ``q`` e4m3 ``[..., F]`` for ``x`` ``[..., 2 F]``;
+    ``scales`` and ``as_rounded`` as in ``rmsnorm_fp8``.  Inference only."""
+    from . import quant
+    if x.shape[-1] % 2:
+        raise ValueError(f"swiglu_fp8: x {tuple(x.shape)} is not [gate | up]")
+    F = x.shape[-1] // 2
+    _check_e4m3_rows("swiglu_fp8", x, F, scales)
+    if not (x.dtype == torch.bfloat16 and _lib.use_native(x)):
+        g, u = x.float().chunk(2, dim=-1)
+        y = torch.nn.functional.silu(g) * u
+        return quant.quant_rows_ref(y.to(x.dtype) if as_rounded else y, scales)
+    with _lib.on_device(x):
+        x2 = _lib.packed16(x)
+        q, s = _e4m3_buffers(x2.numel() // (2 * F), F, scales, x.device)
+        LAUNCHES["elementwise"] += 1
+        _lib.check(_lib.kernels().gk_rows_quant(_lib.ptr(x2), _lib.ptr(q), _lib.ptr(s), q.shape[0], F, 1, scales == "e8m0",
+                                                as_rounded, _lib.stream_ptr()), "rows_quant")
+    return q.view(*x.shape[:-1], F), s.view(*x.shape[:-1], s.shape[1])
+
+
 def decode_begin(st, block: int, embed=None, sink=None):
     """In front of a decode step over the batch state ``st`` (GPU tensors): ``(slots, ctx, states, sink_slots, x)``, the cache
     row of every request's token (-1 where nothing is stored: a row that rests or has reached its limit), the tokens it sees,

@@ -269,3 +269,187 @@ class Fp8Linear(torch.nn.Module):
         y = gemm_fp8_blockscaled(aq, as_, self.weight_q, self.weight_scale, out_dtype=x.dtype
                                  if x.dtype in (torch.bfloat16, torch.float32) else torch.bfloat16)
         return y.reshape(*shp[:-1], self.weight_q.shape[0])
+
+
+# ------------------------------------------------------------------------------------------------ 4-bit weights
+def quant_rows_ref(y: torch.Tensor, scales: str):
+    """``(q, s)`` of the rows of ``y``: e4m3 codes with one fp32 scale per 128 values (``fp32``) or the smallest power of two per
+    32 values that keeps them within 448 (``e8m0``); a group that holds a NaN or an infinity has the exponent of NaN."""
+    if scales == "fp32":
+        q, s = act_quant_1x128_ref(y.reshape(-1, y.shape[-1]))
+        return q.view(y.shape), s.view(*y.shape[:-1], -1)
+    g = y.float().unflatten(-1, (-1, 32))
+    top = g.abs().amax(-1).clamp_min(1e-10)
+    m, e = torch.frexp(torch.where(torch.isfinite(top), top, torch.ones_like(top)))
+    e = e - 9 + (m > 0.875)                     # 448 = 0.875 * 2^9
+    q = torch.ldexp(g, -e[..., None]).clamp(-E4M3_MAX, E4M3_MAX).to(torch.float8_e4m3fn)
+    code = torch.where(torch.isfinite(top), e + 127, torch.full_like(e, 255)).to(torch.uint8)
+    return q.view(y.shape), code.view(torch.float8_e8m0fnu)
+
+
+def quant_act_1x32(x: torch.Tensor):
+    """``x`` [..., K] (K a multiple of 32) -> ``(q float8_e4m3fn [..., K], s float8_e8m0fnu [..., K / 32])``, the activations of
+    ``gemm_fp4``.  No gradient."""
+    K = x.shape[-1]
+    if K == 0 or K % 32:
+        raise ValueError(f"quant_act_1x32: a width of {K} is not a multiple of 32")
+    if not (_lib.use_native(x) and x.dtype == torch.bfloat16):
+        return quant_rows_ref(x.detach(), "e8m0")
+    with _lib.on_device(x):
+        x2 = _lib.packed16(x.detach())
+        q = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=x.device)
+        s = torch.empty(*x.shape[:-1], K // 32, dtype=torch.float8_e8m0fnu, device=x.device)
+        LAUNCHES["quant"] += 1
+        _lib.check(_lib.kernels().gk_rows_quant(_lib.ptr(x2), _lib.ptr(q), _lib.ptr(s), x2.numel() // K, K, 0, 1, 0,
+                                                _lib.stream_ptr()), "rows_quant")
+    return q, s
+
+
+class Fp4Weight:
+    """A frozen projection weight ``[N, K]`` in 4 bits, laid out once for the kernels that read it: e2m1 codes, two a byte with
+    the even column in the low half, and one power of two per 32 columns.  ``codes`` uint8 [N, K / 2] and ``exponents`` (biased
+    by 127; uint8 or float8_e8m0fnu, [N, K / 32]) are what ``quant_fp4_1x32`` makes and what published 4-bit checkpoints hold;
+    ``Fp4Weight.of(w)`` quantises.  K is a multiple of 32."""
+
+    def __init__(self, codes: torch.Tensor, exponents: torch.Tensor):
+        if codes.dtype != torch.uint8 or codes.dim() != 2:
+            raise ValueError(f"Fp4Weight: codes are uint8 [N, K / 2], got {codes.dtype} {tuple(codes.shape)}")
+        N, K = codes.shape[0], 2 * codes.shape[1]
+        if N == 0 or K == 0 or K % 32:
+            raise ValueError(f"Fp4Weight: [{N}, {K}] (rows, and columns in whole groups of 32, are needed)")
+        if exponents.dtype not in (torch.uint8, torch.float8_e8m0fnu) or tuple(exponents.shape) != (N, K // 32):
+            raise ValueError(f"Fp4Weight: exponents are uint8 or float8_e8m0fnu [{N}, {K // 32}], got {exponents.dtype} "
+                             f"{tuple(exponents.shape)}")
+        if exponents.device != codes.device:
+            raise ValueError(f"Fp4Weight: codes on {codes.device}, exponents on {exponents.device}")
+        self.shape, self.device = (N, K), codes.device
+        # columns in whole tiles of 128 (codes behind the last one are zero), rows on 32-byte boundaries
+        self.padded = (K + 127) // 128 * 128
+        if self.padded != K:
+            codes = torch.nn.functional.pad(codes, (0, (self.padded - K) // 2))
+        self.codes = codes if codes.is_contiguous() and codes.data_ptr() % 32 == 0 else codes.clone(
+            memory_format=torch.contiguous_format)
+        # exponents in tiles of 128 rows x 128 columns, 512 bytes: row r at (r % 32) * 16 + (r / 32) * 4
+        nt, kt = (N + 127) // 128, self.padded // 128
+        e = torch.nn.functional.pad(exponents.view(torch.uint8), (0, 4 * kt - K // 32, 0, 128 * nt - N), value=127)
+        self.tiles = e.view(nt, 4, 32, kt, 4).permute(0, 3, 2, 1, 4).contiguous()
+
+    @classmethod
+    def of(cls, w: torch.Tensor) -> "Fp4Weight":
+        """``w`` [N, K] in 4 bits, each group of 32 columns with the power of two of ``quant_fp4_1x32``."""
+        N, K = w.shape
+        if K % 32:
+            raise ValueError(f"Fp4Weight: {K} columns are not whole groups of 32")
+        packed, e8, _ = quant_fp4_1x32(w.detach().contiguous())
+        return cls(packed.view(N, K // 2), e8.view(N, K // 32))
+
+    @property
+    def exponents(self) -> torch.Tensor:
+        """Biased exponents uint8 [N, K / 32]."""
+        nt, kt = self.tiles.shape[:2]
+        return self.tiles.permute(0, 3, 2, 1, 4).reshape(nt * 128, kt * 4)[:self.shape[0], :self.shape[1] // 32]
+
+    def values(self, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+        """The weight [N, K] in ``dtype`` (bf16 holds every value; the result may be a view of wider rows)."""
+        N, K = self.shape
+        if dtype == torch.bfloat16 and _lib.use_native(self.codes):
+            with _lib.on_device(self.codes):
+                out = torch.empty(N, self.padded, dtype=dtype, device=self.device)
+                LAUNCHES["quant"] += 1
+                _lib.check(_lib.kernels().gk_fp4_dequant(_lib.ptr(self.codes), _lib.ptr(self.tiles), _lib.ptr(out), N,
+                                                         self.padded, _lib.stream_ptr()), "fp4_dequant")
+            return out[:, :K]
+        c = torch.stack([self.codes & 15, self.codes >> 4], dim=-1).view(N, self.padded)[:, :K].int()
+        v = E2M1_VALUES.to(self.device)[c & 7] * torch.where(c >= 8, -1.0, 1.0)
+        e = self.exponents.int()
+        scale = torch.where(e == 255, torch.full_like(e, 0, dtype=torch.float32) + float("nan"),
+                            torch.ldexp(torch.ones_like(e, dtype=torch.float32), e - 127))
+        return (v.view(N, K // 32, 32) * scale[..., None]).view(N, K).to(dtype)
+
+
+def _check_fp4(what, x, weight, bias):
+    if not isinstance(weight, Fp4Weight):
+        raise TypeError(f"{what}: weight is an Fp4Weight, got {type(weight).__name__}")
+    N, K = weight.shape
+    if x.dim() == 0 or x.shape[-1] != K:
+        raise ValueError(f"{what}: x {tuple(x.shape)} against a weight {weight.shape}")
+    if x.device != weight.device or (bias is not None and bias.device != x.device):
+        raise ValueError(f"{what}: tensors on {x.device}, {weight.device}" + (f", {bias.device}" if bias is not None else ""))
+    if bias is not None and tuple(bias.shape) != (N,):
+        raise ValueError(f"{what}: bias {tuple(bias.shape)} for {N} outputs")
+
+
+def _fp4_product(x2, weight: Fp4Weight, bias, out_dtype):
+    """``x2`` [T, K] bf16 (contiguous, on a GPU) times the weight."""
+    if x2.shape[0] == 0:
+        return torch.empty(0, weight.shape[0], dtype=out_dtype, device=x2.device)
+    from .gemm import linear_forward
+    return linear_forward(x2, weight.values(), bias, out_dtype=out_dtype)
+
+
+class _LinearFp4(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x2, weight, bias):
+        ctx.weight, ctx.bias_dtype = weight, bias.dtype if bias is not None else None
+        return _fp4_product(x2, weight, bias, x2.dtype)
+
+    @staticmethod
+    def backward(ctx, dy):
+        dx = db = None
+        if ctx.needs_input_grad[0]:
+            from .gemm import linear_dgrad
+            N, K = ctx.weight.shape
+            w = ctx.weight.values()
+            pad = -N % 8   # the product reads rows in 16-byte units
+            if pad:
+                dy8, w = torch.nn.functional.pad(dy, (0, pad)), torch.nn.functional.pad(w, (0, 0, 0, pad))
+            else:
+                dy8 = _lib.packed16(dy)
+            dx = linear_dgrad(dy8, w) if dy.shape[0] else dy.new_empty(0, K)
+        if ctx.needs_input_grad[2]:
+            db = dy.float().sum(0).to(ctx.bias_dtype)
+        return dx, None, db
+
+
+def linear_fp4(x: torch.Tensor, weight: Fp4Weight, bias: torch.Tensor | None = None) -> torch.Tensor:
+    """``y = x W^T (+ bias)`` for a frozen 4-bit weight and 16-bit activations, ``x`` [..., K] -> [..., N] in ``x``'s type: the
+    product that a model trained with ``fp4_qat`` computes.  Differentiable in ``x`` and ``bias``."""
+    _check_fp4("linear_fp4", x, weight, bias)
+    N, K = weight.shape
+    if not (_lib.use_native(x) and x.dtype == torch.bfloat16):
+        y = torch.nn.functional.linear(x.float(), weight.values(torch.float32), bias.float() if bias is not None else None)
+        return y.to(x.dtype)
+    with _lib.on_device(x):
+        x2 = _lib.packed16(x.reshape(-1, K))
+        if torch.is_grad_enabled() and (x.requires_grad or (bias is not None and bias.requires_grad)):
+            y = _LinearFp4.apply(x2, weight, bias)
+        else:
+            y = _fp4_product(x2, weight, bias, x.dtype)
+    return y.view(*x.shape[:-1], N)
+
+
+def gemm_fp4(a_q: torch.Tensor, a_s: torch.Tensor, weight: Fp4Weight, bias: torch.Tensor | None = None,
+             out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """``y = dequant(a_q, a_s) W^T (+ bias)``: e4m3 activations ``a_q`` [..., K] with one power of two per 32 values ``a_s``
+    (float8_e8m0fnu [..., K / 32]; ``rmsnorm_fp8``, ``swiglu_fp8`` and ``quant_act_1x32`` make them) times a 4-bit weight, in
+    ``out_dtype`` (bf16 or fp32).  No gradient."""
+    if a_q.dtype != torch.float8_e4m3fn or a_s.dtype != torch.float8_e8m0fnu:
+        raise ValueError(f"gemm_fp4: activations are float8_e4m3fn with float8_e8m0fnu scales, got {a_q.dtype}, {a_s.dtype}")
+    _check_fp4("gemm_fp4", a_q, weight, bias)
+    N, K = weight.shape
+    if tuple(a_s.shape) != (*a_q.shape[:-1], K // 32) or a_s.device != a_q.device:
+        raise ValueError(f"gemm_fp4: scales {tuple(a_s.shape)} on {a_s.device} for activations {tuple(a_q.shape)} on {a_q.device}")
+    if out_dtype not in (torch.bfloat16, torch.float32):
+        raise ValueError(f"gemm_fp4: results are bfloat16 or float32, not {out_dtype}")
+    if not _lib.use_native(a_q):
+        x = (a_q.float().unflatten(-1, (-1, 32)) * a_s.float()[..., None]).flatten(-2)
+        y = torch.nn.functional.linear(x, weight.values(torch.float32), bias.float() if bias is not None else None)
+        return y.to(out_dtype)
+    with _lib.on_device(a_q):
+        q2, s2 = _lib.packed16(a_q.reshape(-1, K)), a_s.reshape(-1, K // 32).contiguous()
+        x = torch.empty(q2.shape, dtype=torch.bfloat16, device=a_q.device)
+        LAUNCHES["quant"] += 1
+        _lib.check(_lib.kernels().gk_mxfp8_dequant(_lib.ptr(q2), _lib.ptr(s2), _lib.ptr(x), q2.shape[0], K, _lib.stream_ptr()),
+                   "mxfp8_dequant")
+        y = _fp4_product(x, weight, bias, out_dtype)
+    return y.view(*a_q.shape[:-1], N)

@@ -47,11 +47,12 @@ def _populate():
     from . import (attention, conv_norm, depth, diff_attention, fused, gemm, head_prep, latent_attention, matrix_memory, moe,
                    optim, quant, rl, sandwich, scored_attention, streams, vocab, window_attention)
     for mod, names in ((gemm, ("gemm", "grouped_gemm", "grouped_wgrad", "linear")),
-                       (fused, ("rmsnorm", "rope", "swiglu")),
+                       (fused, ("rmsnorm", "rope", "swiglu", "rmsnorm_fp8", "swiglu_fp8")),
                        (attention, ("flash_attn_varlen", "flash_attn_qkvpacked", "paged_decode", "kv_append_rope")),
                        (vocab, ("linear_logprob_entropy", "sample")),
                        (optim, ("adam_step", "sumsq", "axpy_cast")),
-                       (quant, ("quant_act_1x128", "quant_weight_128x128", "quant_fp4_1x32", "gemm_fp8_blockscaled")),
+                       (quant, ("quant_act_1x128", "quant_weight_128x128", "quant_fp4_1x32", "gemm_fp8_blockscaled", "quant_act_1x32", "linear_fp4",
+                                "gemm_fp4")),
                        (sandwich, ("embed_rows", "add_sublayer", "norm_rows")),
                        (window_attention, ("window_attention",)), (matrix_memory, ("matrix_memory", "retention")),
                        (latent_attention, ("latent_attention",)), (depth, ("add_layer",)),

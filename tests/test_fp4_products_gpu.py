@@ -1,0 +1,153 @@
+"""Products with 4-bit weights on the GPU against 64 bits.
+
+Tolerances.  Codes times powers of two are exact in the operands, so what is left is the sum and the result's rounding.  The tensor
+core adds 16 or 32 products at a time to a 32-bit sum, each addition off by at most 2^-23 of what has been added: (K / 16 + 16)
+2^-23 of sum |x w|.  Where 16-bit activations are two e4m3 terms a term's rest below 2^-22 of the largest of its group of 32 is
+lost: 2^-21 of sum (group's largest |x|) |w|.  A bf16 result adds half a step, 2^-8 relative to it (2^-9 for an exact one)."""
+import pytest
+import torch
+
+from gcore_b200.ops import quant
+
+pytestmark = pytest.mark.gpu
+
+
+def rand(*shape, seed=0, scale=1.0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return scale * torch.randn(*shape, generator=g, device="cuda")
+
+
+def weight(N, K, seed=0):
+    # groups of very different size, some of them zero
+    w = rand(N, K // 32, 32, seed=seed) * torch.exp2(torch.randint(-12, 3, (N, K // 32, 1), device="cuda").float())
+    w[:: 5, 0] = 0
+    return quant.Fp4Weight.of(w.view(N, K).bfloat16())
+
+
+def bound(x, w, y, dtype):
+    K = x.shape[1]
+    top = x.abs().unflatten(-1, (-1, 32)).amax(-1, keepdim=True).expand(-1, -1, 32).flatten(-2)
+    b = (K / 16 + 16) * 2.0 ** -23 * (x.abs() @ w.abs().t()) + 2.0 ** -21 * (top @ w.abs().t())
+    return b + (2.0 ** -8 * (y.abs() + b) if dtype == torch.bfloat16 else 0) + 1e-30
+
+
+SIZES = [(1, 128, 32), (1, 300, 3584), (3, 1, 64), (8, 129, 256), (13, 4608, 3584), (16, 513, 1184), (33, 3584, 4128), (64, 896, 18944),
+         (100, 1027, 512), (128, 256, 1536), (129, 640, 1024), (257, 2293, 1056), (1000, 384, 2048)]
+
+
+@pytest.mark.parametrize("T,N,K", SIZES)
+def test_products(T, N, K):
+    W = weight(N, K, seed=N + K)
+    w = W.values(torch.float32).double()
+    x = (rand(T, K, seed=T) * torch.exp(rand(K, seed=1))).bfloat16()
+    bias = rand(N, seed=3).bfloat16()
+    for b in (None, bias, bias.float()):
+        y = x.double() @ w.t() + (b.double() if b is not None else 0)
+        got = quant.linear_fp4(x, W, b)
+        assert got.shape == (T, N) and got.dtype == torch.bfloat16
+        assert ((got.double() - y).abs() <= bound(x.double(), w, y, torch.bfloat16)).all()
+    q, s = quant.quant_act_1x32(x)
+    xq = (q.double().unflatten(-1, (-1, 32)) * s.double()[..., None]).flatten(-2)
+    y = xq @ w.t()
+    for dtype in (torch.bfloat16, torch.float32):
+        got = quant.gemm_fp4(q, s, W, out_dtype=dtype)
+        assert got.dtype == dtype and ((got.double() - y).abs() <= bound(xq, w, y, dtype)).all()
+    got = quant.gemm_fp4(q, s, W, bias)
+    assert ((got.double() - y - bias.double()).abs() <= bound(xq, w, y + bias.double(), torch.bfloat16)).all()
+
+
+def test_every_code_and_column_is_read_once_and_in_order():
+    """One token with a single 1: the product is one column of the weight, exactly."""
+    N, K = 130, 256
+    W = weight(N, K, seed=9)
+    w = W.values(torch.bfloat16)
+    eye = torch.eye(K, device="cuda").bfloat16()
+    assert torch.equal(quant.linear_fp4(eye, W), w.t())
+    for k in (0, 1, 31, 32, 63, 127, 128, 200, 255):
+        assert torch.equal(quant.linear_fp4(eye[k:k + 1], W)[0], w[:, k])
+        q, s = quant.quant_act_1x32(eye[k:k + 1])
+        assert torch.equal(quant.gemm_fp4(q, s, W)[0], w[:, k])
+
+
+@pytest.mark.parametrize("T", [1, 5, 40, 200])
+def test_activations_of_any_size(T):
+    """Outliers, tiny values, zeros and whole rows of nothing; rows do not touch one another."""
+    N, K = 384, 640
+    W = weight(N, K, seed=4)
+    w = W.values(torch.float32).double()
+    x = rand(T, K, seed=6)
+    x[:, 5] *= 3000
+    x[:, 70] = 1e-6
+    x[:, 96:128] = 0
+    x[:, 200:210] *= 1e-20
+    if T > 2:
+        x[1] = 0
+        x[2] *= 1e30
+    x = x.bfloat16()
+    y = x.double() @ w.t()
+    got = quant.linear_fp4(x, W)
+    assert ((got.double() - y).abs() <= bound(x.double(), w, y, torch.bfloat16)).all()
+    if T > 2:
+        assert (got[1] == 0).all()
+        x[2, 3] = float("nan")
+        bad = quant.linear_fp4(x, W)
+        keep = [i for i in range(T) if i != 2]
+        assert bad[2].isnan().all() and torch.equal(bad[keep], got[keep])
+
+
+def test_row_strides_batches_and_empty():
+    W = weight(256, 512, seed=2)
+    x = rand(6, 1024, seed=1).bfloat16()
+    want = quant.linear_fp4(x[:, 3:515].clone(), W)
+    assert torch.equal(quant.linear_fp4(x[:, 3:515], W), want)
+    assert torch.equal(quant.linear_fp4(x[:, 3:515].unflatten(0, (2, 3)), W), want.view(2, 3, 256))
+    assert quant.linear_fp4(x[:0, :512], W).shape == (0, 256)
+    q, s = quant.quant_act_1x32(x[:0, :512])
+    assert quant.gemm_fp4(q, s, W).shape == (0, 256)
+
+
+@pytest.mark.parametrize("T,N,K", [(1, 64, 96), (40, 257, 320), (300, 1024, 512), (513, 130, 1152)])
+def test_gradient(T, N, K):
+    W = weight(N, K, seed=N)
+    w = W.values(torch.float32).double()
+    x = rand(T, K, seed=1).bfloat16().requires_grad_()
+    b = rand(N, seed=2).bfloat16().requires_grad_()
+    dy = rand(T, N, seed=3).bfloat16()
+    gx, gb = torch.autograd.grad(quant.linear_fp4(x, W, b), (x, b), dy)
+    want = dy.double() @ w
+    tol = (N / 16 + 16) * 2.0 ** -23 * (dy.double().abs() @ w.abs()) + 1e-30
+    assert ((gx.double() - want).abs() <= tol + 2.0 ** -8 * (want.abs() + tol)).all()
+    s = dy.double().sum(0)
+    assert ((gb.double() - s).abs() <= 2.0 ** -8 * s.abs() + T * 2.0 ** -23 * dy.double().abs().sum(0)).all()
+    # along a direction: the product is linear, so the difference quotient is the gradient's product with it
+    d = rand(T, K, seed=8).bfloat16()
+    with torch.no_grad():
+        two = (quant.linear_fp4(x + d, W).double() - quant.linear_fp4(x - d, W).double()) / 2
+    lhs, rhs = (two * dy.double()).sum(), (gx.double() * d.double()).sum()
+    x2 = x.detach().double().abs() + d.double().abs()
+    slack = 2.0 ** -7 * ((x2 @ w.abs().t()) * dy.double().abs()).sum() + 2.0 ** -8 * (gx.double().abs() * d.double().abs()).sum()
+    assert (lhs - rhs).abs() <= slack
+
+
+def test_graphs_and_streams_side_by_side():
+    """Two captured graphs and eager calls of the same weight at once: no shared scratch."""
+    W = weight(1536, 2048, seed=3)
+    xs = [rand(t, 2048, seed=t).bfloat16() for t in (1, 16, 40)]
+    want = [quant.linear_fp4(x, W) for x in xs]
+    graphs = []
+    for x in xs[:2]:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            y = quant.linear_fp4(x, W)
+        graphs.append((g, y))
+    streams = [torch.cuda.Stream() for _ in xs]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        with torch.cuda.stream(streams[0]):
+            graphs[0][0].replay()
+        with torch.cuda.stream(streams[1]):
+            graphs[1][0].replay()
+        with torch.cuda.stream(streams[2]):
+            y = quant.linear_fp4(xs[2], W)
+    torch.cuda.synchronize()
+    assert torch.equal(graphs[0][1], want[0]) and torch.equal(graphs[1][1], want[1]) and torch.equal(y, want[2])
