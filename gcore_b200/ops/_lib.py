@@ -7,7 +7,6 @@ silently degrades to eager PyTorch.  ``GCORE_B200_FORCE_EAGER=1`` selects the Py
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import os
 from pathlib import Path
@@ -108,14 +107,9 @@ def stream_ptr():
     return c_void_p(torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice()))
 
 
-def on_device(t: torch.Tensor):
-    """Context in which ``t``'s device is the current one, so that a launch goes to a stream of that device."""
-    if t.get_device() == torch._C._cuda_getDevice():
-        return _HERE_ALREADY
-    return torch.cuda.device(t.device)
-
-
-_HERE_ALREADY = contextlib.nullcontext()
+def is_current(t: torch.Tensor) -> bool:
+    """Whether the device of ``t`` (on a GPU) is the current one, so that launches go to its streams."""
+    return t.get_device() == torch._C._cuda_getDevice()
 
 
 def packed16(t: torch.Tensor) -> torch.Tensor:
@@ -234,6 +228,8 @@ def _declare_kernels(lib: ctypes.CDLL):
     d("gk_rows_quant", [P, P, P, L, I, I, I, I, P])
     d("gk_fp4_dequant", [P, P, P, L, I, P])
     d("gk_mxfp8_dequant", [P, P, P, L, I, P])
+    d("gk_fp4_decode_scratch", [I, I, I], L)
+    d("gk_fp4_decode", [P, P, P, P, P, P, L, I, P, I, I, I, I, I, I, P, P])
     d("gk_mla_expand", [P, P, P, P, I, I, I, I, I, P])
     d("gk_mla_expand_bwd", [P, P, P, P, I, I, I, I, I, P])
     d("gk_latent_append", [P, L, P, P, P, P, I, I, I, F, F, I, P])

@@ -2,11 +2,13 @@
 //
 // The exponents (e8m0) are kept in tiles of 128 rows x 128 columns, 512 bytes each, row tile by row tile: row r of a tile has the
 // four exponents of its columns at byte (r % 32) * 16 + (r / 32) * 4.  K is a multiple of 128 here (padded with zero codes).
+#include "ptx.cuh"
 #include "host_utils.h"
 #include <cuda_bf16.h>
 #include <cuda_fp8.h>
 
 namespace gq4 {
+using namespace gk;
 
 // 2^(e - 127); 255 is NaN.  2^-127 and values below 2^-126 become zero (subnormals are flushed).
 __device__ __forceinline__ float pow2_of(uint32_t e) {
@@ -56,6 +58,343 @@ __global__ void __launch_bounds__(256) mxfp8_dequant_kernel(const uint2* __restr
   }
 }
 
+// ---------------------------------------------------------------------------------------------- few tokens
+// y[T, N] = x[T, K] W[N, K]^T (+ bias) on the block-scaled tensor core (kind::mxf8f6f4), which takes e2m1 and e4m3 operands with
+// one e8m0 exponent per 32 values of K: the codes of the weight go from memory to the product as they are.
+//
+//   * The 128-row tile runs over output features, the tokens are the product's N (swap-AB).
+//   * 16-bit activations enter as two e4m3 terms, x = 2^e (hi + lo / 16) with one e per 32 values: hi keeps four significant bits, lo
+//     the four behind them, so a bf16 value at most 2^14 below its group's largest is exact and a smaller one is off by less
+//     than 2^-22 of that largest.  The terms are separate columns of one product; the epilogue adds them.
+//   * K is divided over a cluster of `ks` CTAs where there are few tiles: CTA r finishes tokens r, r + ks, ..., whose partial sums
+//     the others send it through distributed shared memory in one copy each (stores of 128 bytes a warp took 20 us for 64
+//     tokens); it adds them in the order of the CTAs.
+//
+// The weight's bytes are what bounds it: half a byte a value and a 32nd for the exponents.
+constexpr int BM = 128, BK = 128, UK = 32;
+constexpr int THREADS = 192;
+constexpr int MAX_STAGES = 8;
+constexpr int A_BYTES = BM * BK;      // a row of 128 codes takes 128 bytes in shared memory: 16 codes and 8 bytes of gap a unit
+constexpr int SF_BYTES = 512;         // exponents of 128 rows x 128 columns
+
+struct Fp4Params {
+  int T, Tp, terms, N, kb, ks, stages, cols;   // cols: columns of the product (Tp * terms); kb: K / 128
+  int ring;                                    // bytes of the operands' ring, or of the partial sums that use it later
+  const uint8_t* tiles;                        // weight exponents
+  const uint8_t* sf;                           // activation exponents: [kb, ceil(cols / 128), 512]
+  void* Y;
+  long long ldy;
+  int out_fp32;
+  const void* bias;
+  int bias_fp32;
+  int* err;
+};
+
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)),
+               "l"(src), "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
+}
+// 512 bytes of exponents (32 rows of 16) to four columns of tensor memory, the same for each quarter of the lanes.
+__device__ __forceinline__ void sf_to_tmem(uint32_t taddr, uint32_t smem_addr) {
+  const uint64_t desc = static_cast<uint64_t>((smem_addr & 0x3FFFF) >> 4) | (static_cast<uint64_t>(128 >> 4) << 32) |
+                        (static_cast<uint64_t>(1) << 46);
+  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+}
+__device__ __forceinline__ void umma_mx(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa, uint32_t sfb,
+                                        uint32_t accumulate) {
+  asm volatile(
+      "{\n"
+      ".reg .pred p;\n"
+      "setp.ne.b32 p, %6, 0;\n"
+      "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n"
+      "}\n" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+      : "memory");
+}
+// fmt: 0 = e4m3, 5 = e2m1; exponents are e8m0; `k4` picks the byte of the four exponents that a lane holds per column.
+__device__ __forceinline__ uint32_t mx_idesc(int m, int n, int a_fmt, int b_fmt, int k4) {
+  return (static_cast<uint32_t>(k4) << 4) | (static_cast<uint32_t>(a_fmt) << 7) | (static_cast<uint32_t>(b_fmt) << 10) |
+         (static_cast<uint32_t>(n >> 3) << 17) | (1u << 23) | (static_cast<uint32_t>(m >> 4) << 24) |
+         (static_cast<uint32_t>(k4) << 29);
+}
+__device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t (&r)[8]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+               : "r"(taddr)
+               : "memory");
+}
+__device__ __forceinline__ uint32_t cta_in_cluster() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+__device__ __forceinline__ uint32_t in_cta(uint32_t local, uint32_t cta) {
+  uint32_t at;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(local), "r"(cta));
+  return at;
+}
+// Own shared memory to another CTA's of the cluster; `bar` is that CTA's.
+__device__ __forceinline__ void bulk_send(uint32_t dst, uint32_t src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.shared::cta.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "r"(src),
+               "r"(bytes), "r"(bar)
+               : "memory");
+}
+
+__global__ void __launch_bounds__(THREADS)
+fp4_decode_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX, Fp4Params p) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const int nsf = (p.cols + 127) / 128;
+  const int b_bytes = p.cols * BK;                                    // a multiple of 2048
+  const int stage_bytes = A_BYTES + b_bytes;
+  const int sf_stage = SF_BYTES * (1 + nsf);
+  const int cs = (p.T + p.ks - 1) / p.ks;                             // token columns that a CTA of the cluster finishes
+  float* part = reinterpret_cast<float*>(smem);                       // own partial sums [ks][cs][128], over the finished ring
+  uint8_t* sf_smem = smem + p.ring;                                   // per stage: the weight's 512 bytes, the activations'
+  float* red = reinterpret_cast<float*>(sf_smem + p.stages * sf_stage);   // the other CTAs' [ks][cs][128]
+  uint64_t* full = reinterpret_cast<uint64_t*>(red + (p.ks > 1 ? p.ks * cs * BM : 0));
+  uint64_t* empty = full + MAX_STAGES;
+  uint64_t* tfull = empty + MAX_STAGES;
+  uint64_t* rfull = tfull + 1;
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(rfull + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = p.ks > 1 ? cta_in_cluster() : 0;
+  const int tile = blockIdx.x / p.ks;
+  const int n0 = tile * BM;
+  // K blocks in shares that differ by one at most
+  const int kb0 = static_cast<int>(static_cast<long long>(p.kb) * rank / p.ks);
+  const int kblocks = static_cast<int>(static_cast<long long>(p.kb) * (rank + 1) / p.ks) - kb0;
+  const int acc_cols = (p.cols + 31) & ~31, sf_cols = 4 * (1 + nsf);
+  uint32_t tmem_cols = 32;
+  while (tmem_cols < static_cast<uint32_t>(acc_cols + p.stages * sf_cols)) tmem_cols <<= 1;
+  const uint32_t stage_tx = A_BYTES / 2 + b_bytes + sf_stage;   // the gaps between the codes do not count
+
+  auto load_weight = [&](int s, int kb) {
+    mbar_expect_tx(&full[s], stage_tx);
+    tma_load_2d(smem + s * stage_bytes, &tmW, &full[s], (kb0 + kb) * BK, n0);
+    bulk_load(sf_smem + s * sf_stage, p.tiles + (static_cast<long long>(tile) * p.kb + kb0 + kb) * SF_BYTES, SF_BYTES, &full[s]);
+  };
+  auto load_tokens = [&](int s, int kb) {
+    tma_load_2d(smem + s * stage_bytes + A_BYTES, &tmX, &full[s], (kb0 + kb) * BK, 0);
+    bulk_load(sf_smem + s * sf_stage + SF_BYTES, p.sf + static_cast<long long>(kb0 + kb) * nsf * SF_BYTES, SF_BYTES * nsf, &full[s]);
+  };
+
+  int pre = 0, loaded = 0;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < p.stages; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
+    mbar_init(tfull, 1);
+    mbar_init(rfull, 1);
+    fence_barrier_init();
+    if (p.ks > 1) mbar_expect_tx(rfull, (p.ks - 1) * cs * BM * 4);
+    pre = kblocks < p.stages ? kblocks : p.stages;
+    for (int kb = 0; kb < pre; ++kb) load_weight(kb, kb);   // the weight does not depend on the kernel in front
+    pdl_wait();
+    for (int kb = 0; kb < pre; ++kb) load_tokens(kb, kb);
+  }
+  if (warp == 2) { tmem_alloc(tmem_holder, tmem_cols); tmem_relinquish(); }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *reinterpret_cast<volatile uint32_t*>(tmem_holder);
+  // not before this CTA has its tensor memory: a kernel behind it that took some and then waited for this one would stop both
+  pdl_launch_dependents();
+  if (p.ks > 1) cluster_arrive();   // "this CTA runs"; the wait is in front of what it is sent
+  pdl_wait();
+
+  bool ok = true;
+  if (warp == 0) {
+    pre = __shfl_sync(0xffffffffu, pre, 0);
+    loaded = pre;
+    int s = pre == p.stages ? 0 : pre;
+    uint32_t ph = pre == p.stages ? 1 : 0;
+    for (int kb = pre; kb < kblocks; ++kb) {
+      ok = mbar_wait_warp(&empty[s], ph ^ 1, p.err, ERR_WAIT_EMPTY);
+      if (!ok) break;
+      if (lane == 0) { load_weight(s, kb); load_tokens(s, kb); }
+      __syncwarp();
+      ++loaded;
+      if (++s == p.stages) { s = 0; ph ^= 1; }
+    }
+    if (p.ks > 1) cluster_wait();
+  } else if (warp == 1) {
+    int s = 0;
+    uint32_t ph = 0;
+    for (int kb = 0; kb < kblocks; ++kb) {
+      ok = mbar_wait_warp(&full[s], ph, p.err, ERR_WAIT_FULL);
+      if (!ok) break;
+      tc_fence_after();
+      if (lane == 0) {
+        const uint32_t a = smem_u32(smem + s * stage_bytes), b = a + A_BYTES, f = smem_u32(sf_smem + s * sf_stage);
+        const uint32_t sfa = tmem_base + acc_cols + s * sf_cols, sfb = sfa + 4;
+        sf_to_tmem(sfa, f);
+        for (int j = 0; j < nsf; ++j) sf_to_tmem(sfb + 4 * j, f + SF_BYTES * (1 + j));
+#pragma unroll
+        for (int k4 = 0; k4 < BK / UK; ++k4)
+          umma_mx(tmem_base, make_smem_desc_sw128(a + k4 * UK, 16, 1024), make_smem_desc_sw128(b + k4 * UK, 16, 1024),
+                  mx_idesc(BM, p.cols, 5, 0, k4), sfa, sfb, (kb > 0 || k4 > 0) ? 1u : 0u);
+        umma_commit(&empty[s]);
+        if (kb == kblocks - 1) umma_commit(tfull);
+      }
+      __syncwarp();
+      if (++s == p.stages) { s = 0; ph ^= 1; }
+    }
+    if (!ok) {   // products under way end before the CTA gives its memory back
+      if (lane == 0) umma_commit(tfull);
+      __syncwarp();
+      mbar_land(tfull, 0);
+    }
+    if (p.ks > 1) cluster_wait();
+  } else {
+    const int quad = warp & 3, row = quad * 32 + lane, feat = n0 + row;
+    if (kblocks > 0) {
+      ok = mbar_wait_warp(tfull, 0, p.err, ERR_WAIT_TMEM_FULL) && *reinterpret_cast<volatile int*>(p.err) == 0;
+      ok = __all_sync(0xffffffffu, ok) != 0;
+      tc_fence_after();
+    }
+    const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quad * 32) << 16);
+    float bias = 0.f;
+    if (p.ks == 1 && p.bias && feat < p.N)
+      bias = p.bias_fp32 ? static_cast<const float*>(p.bias)[feat] : __bfloat162float(static_cast<const __nv_bfloat16*>(p.bias)[feat]);
+    if (ok) {
+      int owner = 0, slot = 0;
+      for (int c = 0; c < p.T; c += 8) {
+        uint32_t r[8], l[8];
+        tmem_ld8(taddr + c, r);
+        if (p.terms == 2) tmem_ld8(taddr + p.Tp + c, l);
+        tmem_ld_wait();
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const int tok = c + j;
+          if (tok >= p.T) break;
+          float v = __uint_as_float(r[j]);
+          if (p.terms == 2) v += __uint_as_float(l[j]);
+          if (p.ks > 1) {
+            part[(owner * cs + slot) * BM + row] = v;
+            if (++owner == p.ks) { owner = 0; ++slot; }
+          } else if (feat < p.N) {
+            v += bias;
+            if (p.out_fp32) static_cast<float*>(p.Y)[tok * p.ldy + feat] = v;
+            else static_cast<__nv_bfloat16*>(p.Y)[tok * p.ldy + feat] = __float2bfloat16(v);
+          }
+        }
+      }
+    }
+    if (p.ks > 1) {
+      fence_proxy_async();
+      cluster_wait();   // every CTA of the cluster runs: it may be sent something
+      asm volatile("bar.sync 1, 128;" ::: "memory");
+      // sent whether or not this CTA is well: the others wait for it
+      if (threadIdx.x == 64) {
+        for (int o = 1; o < p.ks; ++o) {
+          const uint32_t to = (rank + o) % p.ks;
+          bulk_send(in_cta(smem_u32(red + static_cast<int>(rank) * cs * BM), to), smem_u32(part + static_cast<int>(to) * cs * BM),
+                    cs * BM * 4, in_cta(smem_u32(rfull), to));
+        }
+      }
+      __syncwarp();
+      const bool got = mbar_wait_warp(rfull, 0, p.err, ERR_WAIT_MISC);
+      if (!got) mbar_land(rfull, 0);
+      ok = __all_sync(0xffffffffu, ok && got && *reinterpret_cast<volatile int*>(p.err) == 0) != 0;
+      if (ok && feat < p.N) {
+        float bias = 0.f;
+        if (p.bias)
+          bias = p.bias_fp32 ? static_cast<const float*>(p.bias)[feat] : __bfloat162float(static_cast<const __nv_bfloat16*>(p.bias)[feat]);
+        for (int j = 0; j * p.ks + static_cast<int>(rank) < p.T; ++j) {
+          const int tok = j * p.ks + rank;
+          float v = 0.f;
+          for (int r = 0; r < p.ks; ++r) v += (r == static_cast<int>(rank) ? part : red)[(r * cs + j) * BM + row];
+          v += bias;
+          if (p.out_fp32) static_cast<float*>(p.Y)[tok * p.ldy + feat] = v;
+          else static_cast<__nv_bfloat16*>(p.Y)[tok * p.ldy + feat] = __float2bfloat16(v);
+        }
+      }
+    }
+    tc_fence_before();
+  }
+  if (p.ks > 1) {   // what this CTA sent has been read: its owners have seen it arrive
+    __syncwarp();
+    cluster_arrive();
+    cluster_wait();
+  }
+  tc_fence_before();
+  const bool failed = __syncthreads_or(!ok);
+  if (failed && warp == 0) {   // and so do copies that nobody waits for any more
+    for (int kb = loaded > p.stages ? loaded - p.stages : 0; kb < loaded; ++kb)
+      mbar_land(&full[kb % p.stages], static_cast<uint32_t>(kb / p.stages) & 1);
+  }
+  if (warp == 2) { tc_fence_after(); tmem_dealloc(tmem_base, tmem_cols); }
+}
+
+// bf16 rows to the two e4m3 terms, eight values a thread: codes [2 Tp, Kp], hi rows first, and exponents in tiles of 128 code rows.
+// Columns from K to Kp become zero.
+__global__ void __launch_bounds__(256) fp4_split_kernel(const uint4* __restrict__ x, uint2* __restrict__ codes,
+                                                        uint8_t* __restrict__ sf, int T, int Tp, int K, int Kp) {
+  pdl_wait();
+  pdl_launch_dependents();   // behind the wait: the product takes tensor memory, which the kernel in front may still want
+  const int per = Kp / 8, live = K / 8, nsf = (2 * Tp + 127) / 128;
+  const long long units = static_cast<long long>(T) * per;   // a multiple of 16
+  for (long long u0 = blockIdx.x * 256ll; u0 < units; u0 += gridDim.x * 256ll) {
+    const long long u = u0 + threadIdx.x;
+    const int t = static_cast<int>(u / per), c = static_cast<int>(u - static_cast<long long>(t) * per);
+    uint4 raw = make_uint4(0, 0, 0, 0);
+    if (u < units && c < live) raw = x[static_cast<long long>(t) * live + c];
+    const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+    float f[8];
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      f[2 * i] = __uint_as_float(w[i] << 16);
+      f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+      top = max(top, max(w[i] & 0x7fffu, (w[i] >> 16) & 0x7fffu));
+    }
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    // bf16 pattern of the largest: eight bits of exponent, seven of mantissa; 448 = 1.75 * 2^8 as in quant_rows.cu.  The lo
+    // term's exponent is four less, so the hi term's is at least 4 (values below 2^-114 lose bits there).
+    uint32_t e = (top >> 7) - 8u + ((top & 0x7fu) > 0x60u ? 1u : 0u);
+    if (top < (13u << 7)) e = 4u;
+    const bool bad = top >= 0x7f80u;
+    const float inv = __uint_as_float((254u - (bad ? 127u : e)) << 23);
+    uint32_t hi[4], lo[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float a = f[2 * i] * inv, b = f[2 * i + 1] * inv;
+      hi[i] = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+      const __half2 h = __half2(__nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(hi[i]), __NV_E4M3));
+      lo[i] = __nv_cvt_float2_to_fp8x2(make_float2((a - __low2float(h)) * 16.f, (b - __high2float(h)) * 16.f), __NV_SATFINITE,
+                                       __NV_E4M3);
+    }
+    if (u < units) {
+      codes[u] = make_uint2(hi[0] | (hi[1] << 16), hi[2] | (hi[3] << 16));
+      codes[static_cast<long long>(Tp) * per + u] = make_uint2(lo[0] | (lo[1] << 16), lo[2] | (lo[3] << 16));
+      if ((c & 3) == 0) {
+        const int kb = c >> 4, k4 = (c >> 2) & 3;
+        uint8_t* at = sf + static_cast<long long>(kb) * nsf * SF_BYTES + k4;
+        const int r = t, q = Tp + t;
+        at[(r >> 7) * SF_BYTES + (r & 31) * 16 + ((r >> 5) & 3) * 4] = static_cast<uint8_t>(bad ? 255u : e);
+        at[(q >> 7) * SF_BYTES + (q & 31) * 16 + ((q >> 5) & 3) * 4] = static_cast<uint8_t>(bad ? 255u : e - 4u);
+      }
+    }
+  }
+}
+
+// Exponents [T, K / 32] to tiles of 128 rows x 128 columns; columns from K to the tile's end get 1.
+__global__ void __launch_bounds__(256) fp4_tiles_kernel(const uint8_t* __restrict__ s, uint8_t* __restrict__ sf, int T, int per,
+                                                        int kb, int nsf) {
+  pdl_wait();
+  pdl_launch_dependents();
+  const long long n = static_cast<long long>(T) * kb * 4;
+  for (long long i = blockIdx.x * 256ll + threadIdx.x; i < n; i += gridDim.x * 256ll) {
+    const int t = static_cast<int>(i / (kb * 4)), c = static_cast<int>(i - static_cast<long long>(t) * kb * 4);
+    sf[(static_cast<long long>(c >> 2) * nsf + (t >> 7)) * SF_BYTES + (t & 31) * 16 + ((t >> 5) & 3) * 4 + (c & 3)] =
+        c < per ? s[static_cast<long long>(t) * per + c] : 127;
+  }
+}
+
 inline unsigned grid_for(long long units) {
   const long long want = (units + 255) / 256, most = gk::sm_count() * 32ll;
   return static_cast<unsigned>(want < most ? want : most);
@@ -81,4 +420,135 @@ GK_EXPORT int gk_mxfp8_dequant(const void* q, const void* e, void* out, long lon
   gq4::mxfp8_dequant_kernel<<<gq4::grid_for(units), 256, 0, static_cast<cudaStream_t>(stream)>>>(
       static_cast<const uint2*>(q), static_cast<const uint8_t*>(e), static_cast<uint4*>(out), units);
   return gk::launch_status();
+}
+
+namespace gq4 {
+
+// Codes [rows, K] (K a multiple of 128) as 128 x 128 tiles whose rows are spread to 128 bytes.
+inline int make_tmap_fp4(CUtensorMap* out, const void* base, uint64_t rows, uint64_t K) {
+  gk::EncodeTiledFn fn = gk::get_encode_fn();
+  if (!fn) return -1;
+  cuuint64_t dims[2] = {K, rows}, strides[1] = {K / 2};
+  cuuint32_t box[2] = {128, 128}, estr[2] = {1, 1};
+  CUresult r = CUDA_SUCCESS;
+  for (int attempt = 0; attempt < 2; ++attempt) {
+    r = fn(out, CU_TENSOR_MAP_DATA_TYPE_16U4_ALIGN16B, 2, const_cast<void*>(base), dims, strides, box, estr,
+           CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_ERROR_INVALID_CONTEXT) break;
+    gk::bind_primary_context();
+  }
+  return r == CUDA_SUCCESS ? 0 : -2;
+}
+
+struct Fp4Plan {
+  int Tp, cols, nsf, ks, stages, ring, smem;
+};
+
+// Tokens in whole columns of the product, how many CTAs share a tile's K, how deep the ring is.  Measured on B200: a K block of
+// a CTA takes 0.3 us for up to 32 columns and 0.5 for 128 (its four products and the copies of exponents in front of them), or
+// its share of the memory's 0.2 us per SM; what is left of a launch, 4 us, every round of CTAs pays.  13 tokens, 4608 x 3584,
+// ks = 1, 2, 4, 8: 18.4, 14.0, 11.0, 11.1 us; 64 tokens, 3584 x 18944: 79, 50, 30, 38.
+inline Fp4Plan plan_for(int T, int terms, int N, int kb) {
+  Fp4Plan p = {};
+  p.Tp = terms == 2 ? (T + 7) / 8 * 8 : (T + 15) / 16 * 16;
+  p.cols = p.Tp * terms;
+  p.nsf = (p.cols + 127) / 128;
+  const int tiles = (N + BM - 1) / BM, sms = gk::sm_count();
+  const int tile_bytes = A_BYTES + p.cols * BK, sf = SF_BYTES * (1 + p.nsf), stage = tile_bytes + sf;
+  float best = 0.f;
+  for (int ks = 1; ks <= 8 && ks <= kb; ks *= 2) {
+    const int share = (kb + ks - 1) / ks, red = ks > 1 ? ks * ((T + ks - 1) / ks) * BM * 4 : 0;
+    const int fixed = 1024 + red + (2 * MAX_STAGES + 3) * 8;
+    int stages = (113 * 1024 - fixed) / stage, resident = 2;   // two CTAs an SM where three stages fit into half of it
+    if (stages < 3) { stages = (224 * 1024 - fixed) / stage; resident = 1; }
+    if (stages > MAX_STAGES) stages = MAX_STAGES;
+    if (stages > share) stages = share;
+    const int ring = stages * tile_bytes > red ? stages * tile_bytes : (red + 1023) / 1024 * 1024;
+    const int smem = ring + stages * sf + fixed;
+    if (stages < 1 || smem > 227 * 1024) continue;
+    const int n = tiles * ks, rounds = (n + sms * resident - 1) / (sms * resident);
+    const float alone = 0.23f + 0.0021f * p.cols, shared = 0.2f * (n > sms ? resident : 1);
+    const float cost = rounds * (4.f + share * (alone > shared ? alone : shared));
+    if (p.ks == 0 || cost < best) {
+      best = cost;
+      p.ks = ks;
+      p.stages = stages;
+      p.ring = ring;
+      p.smem = smem;
+    }
+  }
+  return p;
+}
+
+inline int decode_launch(const void* codes, const void* tiles, const void* xq, long long xq_rows, int xq_cols, const uint8_t* sf,
+                         const Fp4Plan& pl, int T, int terms, int N, int kb, void* Y, long long ldy, int out_fp32, const void* bias,
+                         int bias_fp32, int* err, cudaStream_t st) {
+  CUtensorMap tmW, tmX;
+  if (make_tmap_fp4(&tmW, codes, N, static_cast<uint64_t>(kb) * BK)) return -11;
+  if (gk::make_tmap_2d(&tmX, xq, 1, xq_rows, xq_cols, xq_cols, pl.cols, BK, true)) return -12;
+  Fp4Params p;
+  p.T = T; p.Tp = pl.Tp; p.terms = terms; p.N = N; p.kb = kb; p.ks = pl.ks; p.stages = pl.stages; p.cols = pl.cols; p.ring = pl.ring;
+  p.tiles = static_cast<const uint8_t*>(tiles); p.sf = sf;
+  p.Y = Y; p.ldy = ldy; p.out_fp32 = out_fp32; p.bias = bias; p.bias_fp32 = bias_fp32; p.err = err;
+  static bool configured = false;
+  if (!configured) {
+    if (cudaFuncSetAttribute(fp4_decode_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024) != cudaSuccess) return -13;
+    configured = true;
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((N + BM - 1) / BM * pl.ks, 1, 1);
+  cfg.blockDim = dim3(THREADS, 1, 1);
+  cfg.dynamicSmemBytes = pl.smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = pl.ks;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;   // behind the split kernel of the same call
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  if (cudaLaunchKernelEx(&cfg, fp4_decode_kernel, tmW, tmX, p) != cudaSuccess) return gk::launch_status() ? gk::launch_status() : -14;
+  return gk::launch_status();
+}
+
+}  // namespace gq4
+
+// Bytes of scratch (16-byte aligned) that a call wants.
+GK_EXPORT long long gk_fp4_decode_scratch(int T, int terms, int Kp) {
+  const long long Tp = terms == 2 ? (T + 7) / 8 * 8 : (T + 15) / 16 * 16, cols = Tp * terms;
+  return (terms == 2 ? cols * Kp : 0) + (Kp / 128) * ((cols + 127) / 128) * 512;
+}
+
+// y [T, N] (bf16 or fp32, row stride ldy) of activations and a weight: codes [N, Kp / 2] on a 32-byte boundary, tiles of its
+// exponents.  x: bf16 [T, K] (terms 2) or e4m3 [T, K] with exponents xs [T, K / 32] (terms 1), rows packed, 16-byte aligned;
+// K a multiple of 32, Kp of 128 and less than 128 above it.
+GK_EXPORT int gk_fp4_decode(const void* codes, const void* tiles, const void* x, const void* xs, void* scratch, void* Y,
+                            long long ldy, int out_fp32, const void* bias, int bias_fp32, int T, int terms, int N, int K, int Kp,
+                            int* err, void* stream) {
+  using namespace gq4;
+  if ((terms != 1 && terms != 2) || T < 1 || T > 128 || N < 1 || K < 32 || K % 32 || Kp % 128 || Kp < K ||
+      Kp - K >= 128)
+    return -1;
+  if ((reinterpret_cast<uintptr_t>(codes) & 31) ||
+      ((reinterpret_cast<uintptr_t>(tiles) | reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(scratch)) & 15))
+    return -2;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const int kb = Kp / 128;
+  const Fp4Plan pl = plan_for(T, terms, N, kb);
+  if (pl.ks == 0) return -3;
+  uint8_t* ws = static_cast<uint8_t*>(scratch);
+  if (terms == 2) {
+    uint8_t* sf = ws + static_cast<long long>(pl.cols) * Kp;
+    gk::launch_k(fp4_split_kernel, dim3(grid_for(static_cast<long long>(T) * (Kp / 8))), dim3(256), 0, st,
+                 static_cast<const uint4*>(x), reinterpret_cast<uint2*>(ws), sf, T, pl.Tp, K, Kp);
+    if (int rc = gk::launch_status()) return rc;
+    return decode_launch(codes, tiles, ws, pl.cols, Kp, sf, pl, T, 2, N, kb, Y, ldy, out_fp32, bias, bias_fp32, err, st);
+  }
+  gk::launch_k(fp4_tiles_kernel, dim3(grid_for(static_cast<long long>(T) * kb * 4)), dim3(256), 0, st,
+               static_cast<const uint8_t*>(xs), ws, T, K / 32, kb, pl.nsf);
+  if (int rc = gk::launch_status()) return rc;
+  return decode_launch(codes, tiles, x, T, K, ws, pl, T, 1, N, kb, Y, ldy, out_fp32, bias, bias_fp32, err, st);
 }

@@ -6,7 +6,7 @@ import ctypes
 
 import torch
 
-from . import _lib
+from . import _lib, quant
 
 LAUNCHES = {"elementwise": 0}
 
@@ -327,26 +327,25 @@ def swiglu(x: torch.Tensor, n_rows: torch.Tensor = None) -> torch.Tensor:
 
 
 # ------------------------------------------------------------------------------------------------ rows that end in e4m3
-def _e4m3_buffers(rows, width, scales, device):
-    """Codes and scales of ``[rows, width]`` values: ``fp32`` one 32-bit scale per 128, ``e8m0`` one power of two per 32."""
-    q = torch.empty(rows, width, dtype=torch.float8_e4m3fn, device=device)
+def _scale_buffer(x, width, scales):
+    """Scales of rows of ``width`` values: ``fp32`` one 32-bit scale per 128, ``e8m0`` one power of two per 32."""
     if scales == "fp32":
-        return q, torch.empty(rows, width // 128, dtype=torch.float32, device=device)
-    return q, torch.empty(rows, width // 32, dtype=torch.float8_e8m0fnu, device=device)
+        return torch.empty((*x.shape[:-1], width // 128), dtype=torch.float32, device=x.device)
+    return torch.empty((*x.shape[:-1], width // 32), dtype=torch.float8_e8m0fnu, device=x.device)
 
 
-def _check_e4m3_rows(what, x, width, scales, *others):
+def _check_e4m3_rows(what, width, scales, x, *others):
     if scales not in ("fp32", "e8m0"):
         raise ValueError(f"{what}: scales must be 'fp32' or 'e8m0', got {scales!r}")
     if width == 0 or width % (128 if scales == "fp32" else 32):
         raise ValueError(f"{what}: a width of {width} is not a multiple of {128 if scales == 'fp32' else 32} ({scales} scales)")
+    grads = torch.is_grad_enabled()
     for t in (x, *others):
-        if t is None:
-            continue
-        if t.device != x.device:
-            raise ValueError(f"{what}: tensors on {x.device} and {t.device}")
-        if t.requires_grad and torch.is_grad_enabled():
-            raise RuntimeError(f"{what} has no gradient: call it under torch.no_grad()")
+        if t is not None:
+            if t.device != x.device:
+                raise ValueError(f"{what}: tensors on {x.device} and {t.device}")
+            if grads and t.requires_grad:
+                raise RuntimeError(f"{what} has no gradient: call it under torch.no_grad()")
 
 
 def rmsnorm_fp8(x: torch.Tensor, w: torch.Tensor, eps: float = 1e-6, residual: torch.Tensor | None = None,
@@ -356,51 +355,56 @@ def rmsnorm_fp8(x: torch.Tensor, w: torch.Tensor, eps: float = 1e-6, residual: t
     ``quant.gemm_fp8_blockscaled`` reads; ``"e8m0"``: one power of two per 32 values (``torch.float8_e8m0fnu``), what
     ``quant.gemm_fp4`` reads.  The norm is rounded once, to e4m3; with ``as_rounded`` it is rounded to ``x``'s type first, so that
     ``q`` and ``s`` are those of ``quant_act_1x128(rmsnorm(...)[0])`` bit for bit.  Inference only."""
-    from . import quant
     H = x.shape[-1]
     if w.shape != (H,) or (residual is not None and residual.shape != x.shape):
         raise ValueError(f"rmsnorm_fp8: x {tuple(x.shape)}, gain {tuple(w.shape)}"
                          + (f", residual {tuple(residual.shape)}" if residual is not None else ""))
-    _check_e4m3_rows("rmsnorm_fp8", x, H, scales, w, residual)
-    if not (x.dtype == torch.bfloat16 and w.dtype == torch.bfloat16 and (residual is None or residual.dtype == torch.bfloat16)
-            and _lib.use_native(x) and H <= 16384):
+    _check_e4m3_rows("rmsnorm_fp8", H, scales, x, w, residual)
+    bf16 = torch.bfloat16
+    if not (x.dtype == bf16 and w.dtype == bf16 and (residual is None or residual.dtype == bf16) and H <= 16384
+            and _lib.use_native(x)):
         xs = x if residual is None else (x.float() + residual.float()).to(x.dtype)
         xf = xs.float()
         y = xf * torch.rsqrt(xf.pow(2).mean(-1, keepdim=True) + eps) * w.float()
         q, s = quant.quant_rows_ref(y.to(x.dtype) if as_rounded else y, scales)
         return q, s, xs
-    with _lib.on_device(x):
-        x2, w2 = _lib.packed16(x), _lib.packed16(w)
-        r2 = _lib.packed16(residual) if residual is not None else None
-        T = x2.numel() // H
-        q, s = _e4m3_buffers(T, H, scales, x.device)
-        out = torch.empty_like(x2) if r2 is not None else None
-        LAUNCHES["elementwise"] += 1
-        _lib.check(_lib.kernels().gk_norm_quant(_lib.ptr(x2), _lib.ptr(r2), _lib.ptr(w2), _lib.ptr(q), _lib.ptr(s),
-                                                _lib.ptr(out), T, H, float(eps), scales == "e8m0", as_rounded,
-                                                _lib.stream_ptr()), "norm_quant")
-    return q.view(x.shape), s.view(*x.shape[:-1], s.shape[1]), x if out is None else out
+    if not _lib.is_current(x):
+        with torch.cuda.device(x.device):
+            return rmsnorm_fp8(x, w, eps, residual, scales, as_rounded)
+    x2, w2 = _lib.packed16(x), _lib.packed16(w)
+    q, s = torch.empty_like(x2, dtype=torch.float8_e4m3fn), _scale_buffer(x, H, scales)
+    r2 = out = None
+    if residual is not None:
+        r2, out = _lib.packed16(residual), torch.empty_like(x2)
+    LAUNCHES["elementwise"] += 1
+    _lib.check(_lib.kernels().gk_norm_quant(
+        x2.data_ptr(), r2.data_ptr() if r2 is not None else None, w2.data_ptr(), q.data_ptr(), s.data_ptr(),
+        out.data_ptr() if out is not None else None, x2.numel() // H, H, eps, scales == "e8m0", as_rounded, _lib.stream_ptr()),
+        "norm_quant")
+    return q, s, x if out is None else out
 
 
 def swiglu_fp8(x: torch.Tensor, scales: str = "fp32", as_rounded: bool = False):
     """``swiglu`` whose result is quantised in the same pass: ``(q, s)`` with ``q`` e4m3 ``[..., F]`` for ``x`` ``[..., 2 F]``;
     ``scales`` and ``as_rounded`` as in ``rmsnorm_fp8``.  Inference only."""
-    from . import quant
     if x.shape[-1] % 2:
         raise ValueError(f"swiglu_fp8: x {tuple(x.shape)} is not [gate | up]")
     F = x.shape[-1] // 2
-    _check_e4m3_rows("swiglu_fp8", x, F, scales)
+    _check_e4m3_rows("swiglu_fp8", F, scales, x)
     if not (x.dtype == torch.bfloat16 and _lib.use_native(x)):
         g, u = x.float().chunk(2, dim=-1)
         y = torch.nn.functional.silu(g) * u
         return quant.quant_rows_ref(y.to(x.dtype) if as_rounded else y, scales)
-    with _lib.on_device(x):
-        x2 = _lib.packed16(x)
-        q, s = _e4m3_buffers(x2.numel() // (2 * F), F, scales, x.device)
-        LAUNCHES["elementwise"] += 1
-        _lib.check(_lib.kernels().gk_rows_quant(_lib.ptr(x2), _lib.ptr(q), _lib.ptr(s), q.shape[0], F, 1, scales == "e8m0",
-                                                as_rounded, _lib.stream_ptr()), "rows_quant")
-    return q.view(*x.shape[:-1], F), s.view(*x.shape[:-1], s.shape[1])
+    if not _lib.is_current(x):
+        with torch.cuda.device(x.device):
+            return swiglu_fp8(x, scales, as_rounded)
+    x2 = _lib.packed16(x)
+    q = torch.empty((*x.shape[:-1], F), dtype=torch.float8_e4m3fn, device=x.device)
+    s = _scale_buffer(x, F, scales)
+    LAUNCHES["elementwise"] += 1
+    _lib.check(_lib.kernels().gk_rows_quant(x2.data_ptr(), q.data_ptr(), s.data_ptr(), x2.numel() // (2 * F), F, 1,
+                                            scales == "e8m0", as_rounded, _lib.stream_ptr()), "rows_quant")
+    return q, s
 
 
 def decode_begin(st, block: int, embed=None, sink=None):

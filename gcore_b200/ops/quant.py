@@ -295,13 +295,15 @@ def quant_act_1x32(x: torch.Tensor):
         raise ValueError(f"quant_act_1x32: a width of {K} is not a multiple of 32")
     if not (_lib.use_native(x) and x.dtype == torch.bfloat16):
         return quant_rows_ref(x.detach(), "e8m0")
-    with _lib.on_device(x):
-        x2 = _lib.packed16(x.detach())
-        q = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=x.device)
-        s = torch.empty(*x.shape[:-1], K // 32, dtype=torch.float8_e8m0fnu, device=x.device)
-        LAUNCHES["quant"] += 1
-        _lib.check(_lib.kernels().gk_rows_quant(_lib.ptr(x2), _lib.ptr(q), _lib.ptr(s), x2.numel() // K, K, 0, 1, 0,
-                                                _lib.stream_ptr()), "rows_quant")
+    if not _lib.is_current(x):
+        with torch.cuda.device(x.device):
+            return quant_act_1x32(x)
+    x2 = _lib.packed16(x.detach())
+    q = torch.empty_like(x2, dtype=torch.float8_e4m3fn)
+    s = torch.empty((*x.shape[:-1], K // 32), dtype=torch.float8_e8m0fnu, device=x.device)
+    LAUNCHES["quant"] += 1
+    _lib.check(_lib.kernels().gk_rows_quant(x2.data_ptr(), q.data_ptr(), s.data_ptr(), x2.numel() // K, K, 0, 1, 0,
+                                            _lib.stream_ptr()), "rows_quant")
     return q, s
 
 
@@ -332,7 +334,7 @@ class Fp4Weight:
         # exponents in tiles of 128 rows x 128 columns, 512 bytes: row r at (r % 32) * 16 + (r / 32) * 4
         nt, kt = (N + 127) // 128, self.padded // 128
         e = torch.nn.functional.pad(exponents.view(torch.uint8), (0, 4 * kt - K // 32, 0, 128 * nt - N), value=127)
-        self.tiles = e.view(nt, 4, 32, kt, 4).permute(0, 3, 2, 1, 4).contiguous()
+        self.tiles = _lib.packed16(e.view(nt, 4, 32, kt, 4).permute(0, 3, 2, 1, 4))
 
     @classmethod
     def of(cls, w: torch.Tensor) -> "Fp4Weight":
@@ -353,11 +355,13 @@ class Fp4Weight:
         """The weight [N, K] in ``dtype`` (bf16 holds every value; the result may be a view of wider rows)."""
         N, K = self.shape
         if dtype == torch.bfloat16 and _lib.use_native(self.codes):
-            with _lib.on_device(self.codes):
-                out = torch.empty(N, self.padded, dtype=dtype, device=self.device)
-                LAUNCHES["quant"] += 1
-                _lib.check(_lib.kernels().gk_fp4_dequant(_lib.ptr(self.codes), _lib.ptr(self.tiles), _lib.ptr(out), N,
-                                                         self.padded, _lib.stream_ptr()), "fp4_dequant")
+            if not _lib.is_current(self.codes):
+                with torch.cuda.device(self.device):
+                    return self.values(dtype)
+            out = torch.empty(N, self.padded, dtype=dtype, device=self.device)
+            LAUNCHES["quant"] += 1
+            _lib.check(_lib.kernels().gk_fp4_dequant(self.codes.data_ptr(), self.tiles.data_ptr(), out.data_ptr(), N, self.padded,
+                                                     _lib.stream_ptr()), "fp4_dequant")
             return out[:, :K]
         c = torch.stack([self.codes & 15, self.codes >> 4], dim=-1).view(N, self.padded)[:, :K].int()
         v = E2M1_VALUES.to(self.device)[c & 7] * torch.where(c >= 8, -1.0, 1.0)
@@ -379,10 +383,34 @@ def _check_fp4(what, x, weight, bias):
         raise ValueError(f"{what}: bias {tuple(bias.shape)} for {N} outputs")
 
 
+FP4_DECODE_TOKENS = 128   # most tokens of the product that streams the weight's codes
+
+
+def _fp4_decode(x2, xs, weight: Fp4Weight, bias, out_dtype):
+    """Few tokens: ``x2`` [T, K] bf16, or e4m3 with exponents ``xs`` [T, K / 32] (packed, on a GPU)."""
+    (T, K), N = x2.shape, weight.shape[0]
+    terms = 2 if xs is None else 1
+    lib = _lib.kernels()
+    y = torch.empty(T, N, dtype=out_dtype, device=x2.device)
+    scratch = torch.empty(lib.gk_fp4_decode_scratch(T, terms, weight.padded), dtype=torch.uint8, device=x2.device)
+    if bias is not None:
+        bias = (bias if bias.dtype in (torch.bfloat16, torch.float32) else bias.float()).contiguous()
+    LAUNCHES["quant"] += 2
+    _lib.check(lib.gk_fp4_decode(
+        weight.codes.data_ptr(), weight.tiles.data_ptr(), x2.data_ptr(), xs.data_ptr() if xs is not None else None,
+        scratch.data_ptr(), y.data_ptr(), N, out_dtype == torch.float32, bias.data_ptr() if bias is not None else None,
+        bias is not None and bias.dtype == torch.float32, T, terms, N, K, weight.padded, _lib.err_flag(x2.device).data_ptr(),
+        _lib.stream_ptr()), "fp4_decode")
+    return y
+
+
 def _fp4_product(x2, weight: Fp4Weight, bias, out_dtype):
-    """``x2`` [T, K] bf16 (contiguous, on a GPU) times the weight."""
-    if x2.shape[0] == 0:
+    """``x2`` [T, K] bf16 (packed, on a GPU) times the weight."""
+    T = x2.shape[0]
+    if T == 0:
         return torch.empty(0, weight.shape[0], dtype=out_dtype, device=x2.device)
+    if T <= FP4_DECODE_TOKENS:
+        return _fp4_decode(x2, None, weight, bias, out_dtype)
     from .gemm import linear_forward
     return linear_forward(x2, weight.values(), bias, out_dtype=out_dtype)
 
@@ -419,13 +447,15 @@ def linear_fp4(x: torch.Tensor, weight: Fp4Weight, bias: torch.Tensor | None = N
     if not (_lib.use_native(x) and x.dtype == torch.bfloat16):
         y = torch.nn.functional.linear(x.float(), weight.values(torch.float32), bias.float() if bias is not None else None)
         return y.to(x.dtype)
-    with _lib.on_device(x):
-        x2 = _lib.packed16(x.reshape(-1, K))
-        if torch.is_grad_enabled() and (x.requires_grad or (bias is not None and bias.requires_grad)):
-            y = _LinearFp4.apply(x2, weight, bias)
-        else:
-            y = _fp4_product(x2, weight, bias, x.dtype)
-    return y.view(*x.shape[:-1], N)
+    if not _lib.is_current(x):
+        with torch.cuda.device(x.device):
+            return linear_fp4(x, weight, bias)
+    x2 = _lib.packed16(x if x.dim() == 2 else x.reshape(-1, K))
+    if torch.is_grad_enabled() and (x.requires_grad or (bias is not None and bias.requires_grad)):
+        y = _LinearFp4.apply(x2, weight, bias)
+    else:
+        y = _fp4_product(x2, weight, bias, x.dtype)
+    return y if x.dim() == 2 else y.view(*x.shape[:-1], N)
 
 
 def gemm_fp4(a_q: torch.Tensor, a_s: torch.Tensor, weight: Fp4Weight, bias: torch.Tensor | None = None,
@@ -445,11 +475,17 @@ def gemm_fp4(a_q: torch.Tensor, a_s: torch.Tensor, weight: Fp4Weight, bias: torc
         x = (a_q.float().unflatten(-1, (-1, 32)) * a_s.float()[..., None]).flatten(-2)
         y = torch.nn.functional.linear(x, weight.values(torch.float32), bias.float() if bias is not None else None)
         return y.to(out_dtype)
-    with _lib.on_device(a_q):
-        q2, s2 = _lib.packed16(a_q.reshape(-1, K)), a_s.reshape(-1, K // 32).contiguous()
+    if not _lib.is_current(a_q):
+        with torch.cuda.device(a_q.device):
+            return gemm_fp4(a_q, a_s, weight, bias, out_dtype)
+    flat = a_q.dim() == 2
+    q2, s2 = _lib.packed16(a_q if flat else a_q.reshape(-1, K)), (a_s if flat else a_s.reshape(-1, K // 32)).contiguous()
+    if 1 <= q2.shape[0] <= FP4_DECODE_TOKENS:
+        y = _fp4_decode(q2, s2, weight, bias, out_dtype)
+    else:
         x = torch.empty(q2.shape, dtype=torch.bfloat16, device=a_q.device)
         LAUNCHES["quant"] += 1
-        _lib.check(_lib.kernels().gk_mxfp8_dequant(_lib.ptr(q2), _lib.ptr(s2), _lib.ptr(x), q2.shape[0], K, _lib.stream_ptr()),
+        _lib.check(_lib.kernels().gk_mxfp8_dequant(q2.data_ptr(), s2.data_ptr(), x.data_ptr(), q2.shape[0], K, _lib.stream_ptr()),
                    "mxfp8_dequant")
         y = _fp4_product(x, weight, bias, out_dtype)
-    return y.view(*a_q.shape[:-1], N)
+    return y if flat else y.view(*a_q.shape[:-1], N)
