@@ -62,7 +62,9 @@ __global__ void __launch_bounds__(256) mxfp8_dequant_kernel(const uint2* __restr
 // y[T, N] = x[T, K] W[N, K]^T (+ bias) on the block-scaled tensor core (kind::mxf8f6f4), which takes e2m1 and e4m3 operands with
 // one e8m0 exponent per 32 values of K: the codes of the weight go from memory to the product as they are.
 //
-//   * The 128-row tile runs over output features, the tokens are the product's N (swap-AB).
+//   * The 128-row tile runs over output features, the tokens are the product's N (swap-AB).  A product instruction takes the same 70
+//     cycles for 16 columns as for 128, and its operands' and descriptors' way to the tensor core is what the issuing warp spends
+//     its time on: with one lane in a branch of its own 64 tokens of 3584 x 18944 took 79 us in one piece, now 46.
 //   * 16-bit activations enter as two e4m3 terms, x = 2^e (hi + lo / 16) with one e per 32 values: hi keeps four significant bits, lo
 //     the four behind them, so a bf16 value at most 2^14 below its group's largest is exact and a smaller one is off by less
 //     than 2^-22 of that largest.  The terms are separate columns of one product; the epilogue adds them.
@@ -70,18 +72,28 @@ __global__ void __launch_bounds__(256) mxfp8_dequant_kernel(const uint2* __restr
 //     the others send it through distributed shared memory in one copy each (stores of 128 bytes a warp took 20 us for 64
 //     tokens); it adds them in the order of the CTAs.
 //
-// The weight's bytes are what bounds it: half a byte a value and a 32nd for the exponents.
+// The weight's bytes bound it with a token or two (half a byte a value and a 32nd for the exponents), the tokens' operand on its way
+// out of L2, 16 KB a K block of 64 tokens for 8.7 KB of weight, from a few dozen on.
 constexpr int BM = 128, BK = 128, UK = 32;
-constexpr int THREADS = 192;
+constexpr int THREADS = 320;          // one warp loads, one issues, eight read the result (the first four also prepare tokens)
 constexpr int MAX_STAGES = 8;
 constexpr int A_BYTES = BM * BK;      // a row of 128 codes takes 128 bytes in shared memory: 16 codes and 8 bytes of gap a unit
 constexpr int SF_BYTES = 512;         // exponents of 128 rows x 128 columns
 
+// Where the product's token operand comes from.
+enum Tokens : int {
+  SPLIT = 0,   // the two terms of bf16 rows and their exponents, made by fp4_split_kernel
+  ROWS16 = 1,  // bf16 rows, split into each stage of the ring by four of the epilogue's warps (up to 8 tokens)
+  ROWS8 = 2,   // e4m3 rows; the same warps bring the exponents into place
+};
+
 struct Fp4Params {
   int T, Tp, terms, N, kb, ks, stages, cols;   // cols: columns of the product (Tp * terms); kb: K / 128
+  int K;                                       // columns that the tokens really have
   int ring;                                    // bytes of the operands' ring, or of the partial sums that use it later
   const uint8_t* tiles;                        // weight exponents
-  const uint8_t* sf;                           // activation exponents: [kb, ceil(cols / 128), 512]
+  const void* x;                               // ROWS16: rows
+  const uint8_t* sf;                           // SPLIT: exponents [kb, ceil(cols / 128), 512]; ROWS8: [T, K / 32]
   void* Y;
   long long ldy;
   int out_fp32;
@@ -95,39 +107,54 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
                "l"(src), "r"(bytes), "r"(smem_u32(bar))
                : "memory");
 }
-// 512 bytes of exponents (32 rows of 16) to four columns of tensor memory, the same for each quarter of the lanes.
-__device__ __forceinline__ void sf_to_tmem(uint32_t taddr, uint32_t smem_addr) {
+// The tensor core's instructions of the decode kernel: the whole warp runs up to them and one lane (`go`) issues, so that
+// addresses and descriptors stay in uniform registers.  512 bytes of exponents (32 rows of 16) to four columns of tensor memory,
+// the same for each quarter of the lanes:
+__device__ __forceinline__ void sf_to_tmem(uint32_t go, uint32_t taddr, uint32_t smem_addr) {
   const uint64_t desc = static_cast<uint64_t>((smem_addr & 0x3FFFF) >> 4) | (static_cast<uint64_t>(128 >> 4) << 32) |
                         (static_cast<uint64_t>(1) << 46);
-  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+  asm volatile(
+      "{\n"
+      ".reg .pred q;\n"
+      "setp.ne.b32 q, %2, 0;\n"
+      "@q tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;\n"
+      "}\n" ::"r"(taddr),
+      "l"(desc), "r"(go)
+      : "memory");
 }
-__device__ __forceinline__ void umma_mx(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa, uint32_t sfb,
+__device__ __forceinline__ void umma_mx(uint32_t go, uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa, uint32_t sfb,
                                         uint32_t accumulate) {
   asm volatile(
       "{\n"
-      ".reg .pred p;\n"
+      ".reg .pred p, q;\n"
       "setp.ne.b32 p, %6, 0;\n"
-      "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n"
+      "setp.ne.b32 q, %7, 0;\n"
+      "@q tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n"
       "}\n" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+      "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate), "r"(go)
       : "memory");
 }
-// fmt: 0 = e4m3, 5 = e2m1; exponents are e8m0; `k4` picks the byte of the four exponents that a lane holds per column.
-__device__ __forceinline__ uint32_t mx_idesc(int m, int n, int a_fmt, int b_fmt, int k4) {
-  return (static_cast<uint32_t>(k4) << 4) | (static_cast<uint32_t>(a_fmt) << 7) | (static_cast<uint32_t>(b_fmt) << 10) |
-         (static_cast<uint32_t>(n >> 3) << 17) | (1u << 23) | (static_cast<uint32_t>(m >> 4) << 24) |
-         (static_cast<uint32_t>(k4) << 29);
+__device__ __forceinline__ void umma_commit_if(uint32_t go, uint64_t* bar) {
+  asm volatile(
+      "{\n"
+      ".reg .pred q;\n"
+      "setp.ne.b32 q, %1, 0;\n"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n"
+      "}\n" ::"r"(smem_u32(bar)),
+      "r"(go)
+      : "memory");
+}
+// fmt: 0 = e4m3, 5 = e2m1; exponents are e8m0.  Bits 4 and 29 and the ones above each count the byte of the four exponents that a
+// lane holds per column (B's and A's).
+__device__ __forceinline__ uint32_t mx_idesc(int m, int n, int a_fmt, int b_fmt) {
+  return (static_cast<uint32_t>(a_fmt) << 7) | (static_cast<uint32_t>(b_fmt) << 10) | (static_cast<uint32_t>(n >> 3) << 17) |
+         (1u << 23) | (static_cast<uint32_t>(m >> 4) << 24);
 }
 __device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t (&r)[8]) {
   asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
                : "r"(taddr)
                : "memory");
-}
-__device__ __forceinline__ uint32_t cta_in_cluster() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-  return r;
 }
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
@@ -143,17 +170,57 @@ __device__ __forceinline__ void bulk_send(uint32_t dst, uint32_t src, uint32_t b
                : "memory");
 }
 
+// Eight bf16 values of a group of 32 (four neighbouring lanes; the whole warp calls this) as two e4m3 terms and the exponents of
+// both; 255 where the group holds a NaN or an infinity.
+struct Terms {
+  uint2 hi, lo;
+  uint32_t e_hi, e_lo;
+};
+__device__ __forceinline__ Terms split8(const uint4& raw) {
+  const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) top = max(top, max(w[i] & 0x7fffu, (w[i] >> 16) & 0x7fffu));
+  top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+  top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+  // bf16 pattern of the largest: eight bits of exponent, seven of mantissa; 448 = 1.75 * 2^8 as in quant_rows.cu.  The lo term's
+  // exponent is four less, so the hi term's is at least 4 (values below 2^-114 lose bits there).
+  uint32_t e = (top >> 7) - 8u + ((top & 0x7fu) > 0x60u ? 1u : 0u);
+  if (top < (13u << 7)) e = 4u;
+  const bool bad = top >= 0x7f80u;
+  const float inv = __uint_as_float((254u - (bad ? 127u : e)) << 23);
+  uint32_t hi[4], lo[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float a = __uint_as_float(w[i] << 16) * inv, b = __uint_as_float(w[i] & 0xffff0000u) * inv;
+    hi[i] = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+    const __half2 h = __half2(__nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(hi[i]), __NV_E4M3));
+    lo[i] = __nv_cvt_float2_to_fp8x2(make_float2((a - __low2float(h)) * 16.f, (b - __high2float(h)) * 16.f), __NV_SATFINITE,
+                                     __NV_E4M3);
+  }
+  Terms t;
+  t.hi = make_uint2(hi[0] | (hi[1] << 16), hi[2] | (hi[3] << 16));
+  t.lo = make_uint2(lo[0] | (lo[1] << 16), lo[2] | (lo[3] << 16));
+  t.e_hi = bad ? 255u : e;
+  t.e_lo = bad ? 255u : e - 4u;
+  return t;
+}
+// Byte of exponent k4 of row r in tiles of 128 rows x 128 columns.
+__device__ __forceinline__ int sf_at(int r, int k4) { return (r >> 7) * SF_BYTES + (r & 31) * 16 + ((r >> 5) & 3) * 4 + k4; }
+
+// SRC: Tokens.  UNITS (ROWS16): units of eight values per lane of a preparing warp and K block, two tokens each.
+template <int SRC, int UNITS>
 __global__ void __launch_bounds__(THREADS)
 fp4_decode_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX, Fp4Params p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  const int nsf = (p.cols + 127) / 128;
+  const int nsf = (p.cols + 127) / 128, ks_log = 31 - __clz(p.ks);    // ks is 1, 2, 4 or 8
   const int b_bytes = p.cols * BK;                                    // a multiple of 2048
   const int stage_bytes = A_BYTES + b_bytes;
   const int sf_stage = SF_BYTES * (1 + nsf);
   const int cs = (p.T + p.ks - 1) / p.ks;                             // token columns that a CTA of the cluster finishes
   float* part = reinterpret_cast<float*>(smem);                       // own partial sums [ks][cs][128], over the finished ring
-  uint8_t* sf_smem = smem + p.ring;                                   // per stage: the weight's 512 bytes, the activations'
+  uint8_t* sf_smem = smem + p.ring;                                   // per stage: the weight's exponents, the tokens'
   float* red = reinterpret_cast<float*>(sf_smem + p.stages * sf_stage);   // the other CTAs' [ks][cs][128]
   uint64_t* full = reinterpret_cast<uint64_t*>(red + (p.ks > 1 ? p.ks * cs * BM : 0));
   uint64_t* empty = full + MAX_STAGES;
@@ -162,7 +229,7 @@ fp4_decode_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(rfull + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t rank = p.ks > 1 ? cta_in_cluster() : 0;
+  const uint32_t rank = blockIdx.x % p.ks;   // in the cluster
   const int tile = blockIdx.x / p.ks;
   const int n0 = tile * BM;
   // K blocks in shares that differ by one at most
@@ -171,7 +238,8 @@ fp4_decode_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant
   const int acc_cols = (p.cols + 31) & ~31, sf_cols = 4 * (1 + nsf);
   uint32_t tmem_cols = 32;
   while (tmem_cols < static_cast<uint32_t>(acc_cols + p.stages * sf_cols)) tmem_cols <<= 1;
-  const uint32_t stage_tx = A_BYTES / 2 + b_bytes + sf_stage;   // the gaps between the codes do not count
+  // the gaps between the codes do not count
+  const uint32_t stage_tx = A_BYTES / 2 + SF_BYTES + (SRC == ROWS16 ? 0 : b_bytes) + (SRC == SPLIT ? nsf * SF_BYTES : 0);
 
   auto load_weight = [&](int s, int kb) {
     mbar_expect_tx(&full[s], stage_tx);
@@ -179,19 +247,21 @@ fp4_decode_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant
     bulk_load(sf_smem + s * sf_stage, p.tiles + (static_cast<long long>(tile) * p.kb + kb0 + kb) * SF_BYTES, SF_BYTES, &full[s]);
   };
   auto load_tokens = [&](int s, int kb) {
-    tma_load_2d(smem + s * stage_bytes + A_BYTES, &tmX, &full[s], (kb0 + kb) * BK, 0);
-    bulk_load(sf_smem + s * sf_stage + SF_BYTES, p.sf + static_cast<long long>(kb0 + kb) * nsf * SF_BYTES, SF_BYTES * nsf, &full[s]);
+    if (SRC != ROWS16) tma_load_2d(smem + s * stage_bytes + A_BYTES, &tmX, &full[s], (kb0 + kb) * BK, 0);
+    if (SRC == SPLIT)
+      bulk_load(sf_smem + s * sf_stage + SF_BYTES, p.sf + static_cast<long long>(kb0 + kb) * nsf * SF_BYTES, SF_BYTES * nsf, &full[s]);
   };
 
   int pre = 0, loaded = 0;
   if (threadIdx.x == 0) {
-    for (int s = 0; s < p.stages; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
+    for (int s = 0; s < p.stages; ++s) { mbar_init(&full[s], SRC == SPLIT ? 1 : 2); mbar_init(&empty[s], 1); }
     mbar_init(tfull, 1);
     mbar_init(rfull, 1);
     fence_barrier_init();
     if (p.ks > 1) mbar_expect_tx(rfull, (p.ks - 1) * cs * BM * 4);
     pre = kblocks < p.stages ? kblocks : p.stages;
-    for (int kb = 0; kb < pre; ++kb) load_weight(kb, kb);   // the weight does not depend on the kernel in front
+    // the weight does not depend on the kernel in front
+    for (int kb = 0; kb < pre; ++kb) load_weight(kb, kb);
     pdl_wait();
     for (int kb = 0; kb < pre; ++kb) load_tokens(kb, kb);
   }
@@ -221,72 +291,154 @@ fp4_decode_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant
     }
     if (p.ks > 1) cluster_wait();
   } else if (warp == 1) {
+    const uint32_t go = elect_one() ? 1 : 0, idesc = mx_idesc(BM, p.cols, 5, 0);
     int s = 0;
     uint32_t ph = 0;
     for (int kb = 0; kb < kblocks; ++kb) {
       ok = mbar_wait_warp(&full[s], ph, p.err, ERR_WAIT_FULL);
       if (!ok) break;
       tc_fence_after();
-      if (lane == 0) {
-        const uint32_t a = smem_u32(smem + s * stage_bytes), b = a + A_BYTES, f = smem_u32(sf_smem + s * sf_stage);
-        const uint32_t sfa = tmem_base + acc_cols + s * sf_cols, sfb = sfa + 4;
-        sf_to_tmem(sfa, f);
-        for (int j = 0; j < nsf; ++j) sf_to_tmem(sfb + 4 * j, f + SF_BYTES * (1 + j));
+      const uint32_t a = smem_u32(smem + s * stage_bytes), b = a + A_BYTES, f = smem_u32(sf_smem + s * sf_stage);
+      const uint32_t sfa = tmem_base + acc_cols + s * sf_cols, sfb = sfa + 4;
+      for (int j = 0; j < 1 + nsf; ++j) sf_to_tmem(go, sfa + 4 * j, f + SF_BYTES * j);
 #pragma unroll
-        for (int k4 = 0; k4 < BK / UK; ++k4)
-          umma_mx(tmem_base, make_smem_desc_sw128(a + k4 * UK, 16, 1024), make_smem_desc_sw128(b + k4 * UK, 16, 1024),
-                  mx_idesc(BM, p.cols, 5, 0, k4), sfa, sfb, (kb > 0 || k4 > 0) ? 1u : 0u);
-        umma_commit(&empty[s]);
-        if (kb == kblocks - 1) umma_commit(tfull);
-      }
-      __syncwarp();
+      for (int k4 = 0; k4 < BK / UK; ++k4)
+        umma_mx(go, tmem_base, make_smem_desc_sw128(a + k4 * UK, 16, 1024), make_smem_desc_sw128(b + k4 * UK, 16, 1024),
+                idesc + k4 * ((1u << 4) + (1u << 29)), sfa, sfb, (kb > 0 || k4 > 0) ? 1u : 0u);
+      umma_commit_if(go, &empty[s]);
+      if (kb == kblocks - 1) umma_commit_if(go, tfull);
       if (++s == p.stages) { s = 0; ph ^= 1; }
     }
     if (!ok) {   // products under way end before the CTA gives its memory back
-      if (lane == 0) umma_commit(tfull);
-      __syncwarp();
+      umma_commit_if(go, tfull);
       mbar_land(tfull, 0);
     }
     if (p.ks > 1) cluster_wait();
   } else {
-    const int quad = warp & 3, row = quad * 32 + lane, feat = n0 + row;
-    if (kblocks > 0) {
-      ok = mbar_wait_warp(tfull, 0, p.err, ERR_WAIT_TMEM_FULL) && *reinterpret_cast<volatile int*>(p.err) == 0;
-      ok = __all_sync(0xffffffffu, ok) != 0;
-      tc_fence_after();
+    // A K block's tokens are one warp's: its chain of load, split, store and fence takes 0.4 us, so four blocks are under way at a
+    // time, and each warp has its next block's loads in flight.  Never more warps than stages: a warp's last block is then at most
+    // a round of the ring behind, and the parity of a stage's barrier tells it whether the stage is free.
+    const int workers = p.stages < 4 ? p.stages : 4;
+    if (SRC == ROWS16 && warp - 2 < workers) {
+      constexpr int U = UNITS > 0 ? UNITS : 1;
+      const __nv_bfloat16* x = static_cast<const __nv_bfloat16*>(p.x);
+      const int c = lane & 15, t0 = lane >> 4;   // unit j: token 2 j + t0, eight values from column 8 c
+      uint4 raw[U];
+      auto fetch = [&](int kb) {
+        const int col = (kb0 + kb) * BK + c * 8;
+#pragma unroll
+        for (int j = 0; j < U; ++j) {
+          const int t = 2 * j + t0;
+          raw[j] = kb < kblocks && t < p.T && col < p.K ? *reinterpret_cast<const uint4*>(x + static_cast<long long>(t) * p.K + col)
+                                                        : make_uint4(0, 0, 0, 0);
+        }
+      };
+      fetch(warp - 2);
+      int s = warp - 2;
+      uint32_t ph = 0;
+      for (int kb = warp - 2; kb < kblocks; kb += workers, s += workers) {
+        while (s >= p.stages) { s -= p.stages; ph ^= 1; }
+        Terms v[U];
+#pragma unroll
+        for (int j = 0; j < U; ++j) v[j] = split8(raw[j]);
+        fetch(kb + workers);
+        ok = mbar_wait_warp(&empty[s], ph ^ 1, p.err, ERR_WAIT_EMPTY);
+        if (!ok) break;
+        uint8_t* b = smem + s * stage_bytes + A_BYTES;
+        uint8_t* f = sf_smem + s * sf_stage + SF_BYTES;
+#pragma unroll
+        for (int j = 0; j < U; ++j) {
+          const int t = 2 * j + t0, l = p.Tp + t;
+          if (t >= p.T) continue;
+          // 16-byte piece c / 2 of the row, in the order of the 128-byte swizzle
+          *reinterpret_cast<uint2*>(b + t * BK + (((c >> 1) ^ (t & 7)) << 4) + (c & 1) * 8) = v[j].hi;
+          *reinterpret_cast<uint2*>(b + l * BK + (((c >> 1) ^ (l & 7)) << 4) + (c & 1) * 8) = v[j].lo;
+          if ((c & 3) == 0) {
+            f[sf_at(t, c >> 2)] = static_cast<uint8_t>(v[j].e_hi);
+            f[sf_at(l, c >> 2)] = static_cast<uint8_t>(v[j].e_lo);
+          }
+        }
+        fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&full[s]);
+      }
+    } else if (SRC == ROWS8 && warp - 2 < workers) {
+      const int per = p.K / 32;
+      uint32_t w[4], next[4];
+      auto fetch = [&](uint32_t (&to)[4], int kb) {   // exponents of a K block for tokens lane, lane + 32, ...; 1 behind the last column
+        const int at = (kb0 + kb) * 4;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int t = lane + 32 * j;
+          to[j] = 0;
+          if (t >= p.T || kb >= kblocks) continue;
+          const uint8_t* mine = p.sf + static_cast<long long>(t) * per + at;
+          if ((per & 3) == 0) {
+            to[j] = *reinterpret_cast<const uint32_t*>(mine);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) to[j] |= (at + i < per ? mine[i] : 127u) << (8 * i);
+          }
+        }
+      };
+      fetch(w, warp - 2);
+      fetch(next, warp - 2 + workers);
+      int s = warp - 2;
+      uint32_t ph = 0;
+      for (int kb = warp - 2; kb < kblocks; kb += workers, s += workers) {
+        while (s >= p.stages) { s -= p.stages; ph ^= 1; }
+        ok = mbar_wait_warp(&empty[s], ph ^ 1, p.err, ERR_WAIT_EMPTY);
+        if (!ok) break;
+        uint8_t* f = sf_smem + s * sf_stage + SF_BYTES;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if (lane + 32 * j < p.T) *reinterpret_cast<uint32_t*>(f + sf_at(lane + 32 * j, 0)) = w[j];
+          w[j] = next[j];
+        }
+        fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&full[s]);
+        fetch(next, kb + 2 * workers);
+      }
     }
+    // Epilogue: a lane per output feature; the warps of the two halves take eight tokens in turn.
+    const int quad = warp & 3, half = (warp - 2) >> 2, row = quad * 32 + lane, feat = n0 + row;
+    ok = ok && mbar_wait_warp(tfull, 0, p.err, ERR_WAIT_TMEM_FULL) && *reinterpret_cast<volatile int*>(p.err) == 0;
+    ok = __all_sync(0xffffffffu, ok) != 0;
+    tc_fence_after();
     const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quad * 32) << 16);
     float bias = 0.f;
-    if (p.ks == 1 && p.bias && feat < p.N)
+    if (p.bias && feat < p.N)
       bias = p.bias_fp32 ? static_cast<const float*>(p.bias)[feat] : __bfloat162float(static_cast<const __nv_bfloat16*>(p.bias)[feat]);
+    auto store = [&](int tok, float v) {
+      if (p.out_fp32) static_cast<float*>(p.Y)[tok * p.ldy + feat] = v;
+      else static_cast<__nv_bfloat16*>(p.Y)[tok * p.ldy + feat] = __float2bfloat16(v);
+    };
     if (ok) {
-      int owner = 0, slot = 0;
-      for (int c = 0; c < p.T; c += 8) {
-        uint32_t r[8], l[8];
-        tmem_ld8(taddr + c, r);
-        if (p.terms == 2) tmem_ld8(taddr + p.Tp + c, l);
+      for (int c = half * 16; c < p.T; c += 32) {
+        uint32_t r[2][8], l[2][8];   // sixteen tokens a wait
+        tmem_ld8(taddr + c, r[0]);
+        if (c + 8 < p.T) tmem_ld8(taddr + c + 8, r[1]);
+        if (p.terms == 2) {
+          tmem_ld8(taddr + p.Tp + c, l[0]);
+          if (c + 8 < p.T) tmem_ld8(taddr + p.Tp + c + 8, l[1]);
+        }
         tmem_ld_wait();
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
+        for (int j = 0; j < 16; ++j) {
           const int tok = c + j;
           if (tok >= p.T) break;
-          float v = __uint_as_float(r[j]);
-          if (p.terms == 2) v += __uint_as_float(l[j]);
-          if (p.ks > 1) {
-            part[(owner * cs + slot) * BM + row] = v;
-            if (++owner == p.ks) { owner = 0; ++slot; }
-          } else if (feat < p.N) {
-            v += bias;
-            if (p.out_fp32) static_cast<float*>(p.Y)[tok * p.ldy + feat] = v;
-            else static_cast<__nv_bfloat16*>(p.Y)[tok * p.ldy + feat] = __float2bfloat16(v);
-          }
+          float v = __uint_as_float(r[j >> 3][j & 7]);
+          if (p.terms == 2) v += __uint_as_float(l[j >> 3][j & 7]);
+          if (p.ks > 1) part[((tok & (p.ks - 1)) * cs + (tok >> ks_log)) * BM + row] = v;
+          else if (feat < p.N) store(tok, v + bias);
         }
       }
     }
     if (p.ks > 1) {
       fence_proxy_async();
       cluster_wait();   // every CTA of the cluster runs: it may be sent something
-      asm volatile("bar.sync 1, 128;" ::: "memory");
+      asm volatile("bar.sync 1, 256;" ::: "memory");
       // sent whether or not this CTA is well: the others wait for it
       if (threadIdx.x == 64) {
         for (int o = 1; o < p.ks; ++o) {
@@ -300,16 +452,10 @@ fp4_decode_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant
       if (!got) mbar_land(rfull, 0);
       ok = __all_sync(0xffffffffu, ok && got && *reinterpret_cast<volatile int*>(p.err) == 0) != 0;
       if (ok && feat < p.N) {
-        float bias = 0.f;
-        if (p.bias)
-          bias = p.bias_fp32 ? static_cast<const float*>(p.bias)[feat] : __bfloat162float(static_cast<const __nv_bfloat16*>(p.bias)[feat]);
-        for (int j = 0; j * p.ks + static_cast<int>(rank) < p.T; ++j) {
-          const int tok = j * p.ks + rank;
+        for (int j = half; j * p.ks + static_cast<int>(rank) < p.T; j += 2) {
           float v = 0.f;
           for (int r = 0; r < p.ks; ++r) v += (r == static_cast<int>(rank) ? part : red)[(r * cs + j) * BM + row];
-          v += bias;
-          if (p.out_fp32) static_cast<float*>(p.Y)[tok * p.ldy + feat] = v;
-          else static_cast<__nv_bfloat16*>(p.Y)[tok * p.ldy + feat] = __float2bfloat16(v);
+          store(j * p.ks + rank, v + bias);
         }
       }
     }
@@ -322,14 +468,14 @@ fp4_decode_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant
   }
   tc_fence_before();
   const bool failed = __syncthreads_or(!ok);
-  if (failed && warp == 0) {   // and so do copies that nobody waits for any more
+  if (failed && warp == 0) {   // copies that nobody waits for any more land before the CTA gives its memory back
     for (int kb = loaded > p.stages ? loaded - p.stages : 0; kb < loaded; ++kb)
       mbar_land(&full[kb % p.stages], static_cast<uint32_t>(kb / p.stages) & 1);
   }
   if (warp == 2) { tc_fence_after(); tmem_dealloc(tmem_base, tmem_cols); }
 }
 
-// bf16 rows to the two e4m3 terms, eight values a thread: codes [2 Tp, Kp], hi rows first, and exponents in tiles of 128 code rows.
+// bf16 rows to their terms, eight values a thread: codes [2 Tp, Kp], hi rows first, and exponents in tiles of 128 code rows.
 // Columns from K to Kp become zero.
 __global__ void __launch_bounds__(256) fp4_split_kernel(const uint4* __restrict__ x, uint2* __restrict__ codes,
                                                         uint8_t* __restrict__ sf, int T, int Tp, int K, int Kp) {
@@ -342,56 +488,16 @@ __global__ void __launch_bounds__(256) fp4_split_kernel(const uint4* __restrict_
     const int t = static_cast<int>(u / per), c = static_cast<int>(u - static_cast<long long>(t) * per);
     uint4 raw = make_uint4(0, 0, 0, 0);
     if (u < units && c < live) raw = x[static_cast<long long>(t) * live + c];
-    const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
-    float f[8];
-    uint32_t top = 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      f[2 * i] = __uint_as_float(w[i] << 16);
-      f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-      top = max(top, max(w[i] & 0x7fffu, (w[i] >> 16) & 0x7fffu));
-    }
-    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-    top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-    // bf16 pattern of the largest: eight bits of exponent, seven of mantissa; 448 = 1.75 * 2^8 as in quant_rows.cu.  The lo
-    // term's exponent is four less, so the hi term's is at least 4 (values below 2^-114 lose bits there).
-    uint32_t e = (top >> 7) - 8u + ((top & 0x7fu) > 0x60u ? 1u : 0u);
-    if (top < (13u << 7)) e = 4u;
-    const bool bad = top >= 0x7f80u;
-    const float inv = __uint_as_float((254u - (bad ? 127u : e)) << 23);
-    uint32_t hi[4], lo[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float a = f[2 * i] * inv, b = f[2 * i + 1] * inv;
-      hi[i] = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
-      const __half2 h = __half2(__nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(hi[i]), __NV_E4M3));
-      lo[i] = __nv_cvt_float2_to_fp8x2(make_float2((a - __low2float(h)) * 16.f, (b - __high2float(h)) * 16.f), __NV_SATFINITE,
-                                       __NV_E4M3);
-    }
+    const Terms v = split8(raw);
     if (u < units) {
-      codes[u] = make_uint2(hi[0] | (hi[1] << 16), hi[2] | (hi[3] << 16));
-      codes[static_cast<long long>(Tp) * per + u] = make_uint2(lo[0] | (lo[1] << 16), lo[2] | (lo[3] << 16));
+      codes[u] = v.hi;
+      codes[static_cast<long long>(Tp) * per + u] = v.lo;
       if ((c & 3) == 0) {
-        const int kb = c >> 4, k4 = (c >> 2) & 3;
-        uint8_t* at = sf + static_cast<long long>(kb) * nsf * SF_BYTES + k4;
-        const int r = t, q = Tp + t;
-        at[(r >> 7) * SF_BYTES + (r & 31) * 16 + ((r >> 5) & 3) * 4] = static_cast<uint8_t>(bad ? 255u : e);
-        at[(q >> 7) * SF_BYTES + (q & 31) * 16 + ((q >> 5) & 3) * 4] = static_cast<uint8_t>(bad ? 255u : e - 4u);
+        uint8_t* at = sf + static_cast<long long>(c >> 4) * nsf * SF_BYTES;
+        at[sf_at(t, (c >> 2) & 3)] = static_cast<uint8_t>(v.e_hi);
+        at[sf_at(Tp + t, (c >> 2) & 3)] = static_cast<uint8_t>(v.e_lo);
       }
     }
-  }
-}
-
-// Exponents [T, K / 32] to tiles of 128 rows x 128 columns; columns from K to the tile's end get 1.
-__global__ void __launch_bounds__(256) fp4_tiles_kernel(const uint8_t* __restrict__ s, uint8_t* __restrict__ sf, int T, int per,
-                                                        int kb, int nsf) {
-  pdl_wait();
-  pdl_launch_dependents();
-  const long long n = static_cast<long long>(T) * kb * 4;
-  for (long long i = blockIdx.x * 256ll + threadIdx.x; i < n; i += gridDim.x * 256ll) {
-    const int t = static_cast<int>(i / (kb * 4)), c = static_cast<int>(i - static_cast<long long>(t) * kb * 4);
-    sf[(static_cast<long long>(c >> 2) * nsf + (t >> 7)) * SF_BYTES + (t & 31) * 16 + ((t >> 5) & 3) * 4 + (c & 3)] =
-        c < per ? s[static_cast<long long>(t) * per + c] : 127;
   }
 }
 
@@ -441,63 +547,78 @@ inline int make_tmap_fp4(CUtensorMap* out, const void* base, uint64_t rows, uint
   return r == CUDA_SUCCESS ? 0 : -2;
 }
 
+typedef void (*DecodeKernel)(CUtensorMap, CUtensorMap, Fp4Params);
+
+inline DecodeKernel decode_kernel(int src, int T) {
+  if (src == SPLIT) return fp4_decode_kernel<SPLIT, 0>;
+  if (src == ROWS8) return fp4_decode_kernel<ROWS8, 0>;
+  return T <= 2 ? fp4_decode_kernel<ROWS16, 1> : fp4_decode_kernel<ROWS16, 4>;
+}
+
 struct Fp4Plan {
-  int Tp, cols, nsf, ks, stages, ring, smem;
+  int Tp, cols, nsf, src, ks, stages, ring, smem;
+  float cost;
 };
 
-// Tokens in whole columns of the product, how many CTAs share a tile's K, how deep the ring is.  Measured on B200: a K block of
-// a CTA takes 0.3 us for up to 32 columns and 0.5 for 128 (its four products and the copies of exponents in front of them), or
-// its share of the memory's 0.2 us per SM; what is left of a launch, 4 us, every round of CTAs pays.  13 tokens, 4608 x 3584,
-// ks = 1, 2, 4, 8: 18.4, 14.0, 11.0, 11.1 us; 64 tokens, 3584 x 18944: 79, 50, 30, 38.
+// Tokens in whole columns of the product, how many CTAs share a tile's K, how deep the ring is: the cheapest by a model of what was
+// measured (B200, us).  A K block of a lone CTA takes 0.26 (the issuing warp's chain) or 0.0085 a KB of operands (60 bytes a
+// cycle, what an SM gets out of L2); two CTAs on an SM share its 0.2 of the memory's rate.  A round of CTAs costs 2, the
+// epilogue 2 + T / 50, the exchange in a cluster 2 + T / 33 and 1 more for eight CTAs, of which fewer fit into a GPC.  Chosen
+// against the others that were run, ks = 1 / 2 / 4 / 8: 1 x 4608 x 3584 12.0 / 9.5 / [9.0] / 9.8, 64 x 4608 x 3584 [14.1] / 14.6 / 21.0 /
+// 26.1, 64 x 3584 x 18944 45.7 / 31.8 / [20.6] / 27.6, 16 x 3584 x 18944 - / 25.4 / 16.7 / [15.2], 96 x 28672 x 4096 (e4m3) [23.1] / 67 / 89 /
+// 154; one or two CTAs an SM: 1 x 37888 x 3584 22.6 / [16.0], 64 x 4608 x 3584 [14.1] / 16.3.
 inline Fp4Plan plan_for(int T, int terms, int N, int kb) {
-  Fp4Plan p = {};
+  Fp4Plan p = {}, best = {};
   p.Tp = terms == 2 ? (T + 7) / 8 * 8 : (T + 15) / 16 * 16;
   p.cols = p.Tp * terms;
   p.nsf = (p.cols + 127) / 128;
+  p.src = terms == 1 ? ROWS8 : T <= 8 ? ROWS16 : SPLIT;
   const int tiles = (N + BM - 1) / BM, sms = gk::sm_count();
   const int tile_bytes = A_BYTES + p.cols * BK, sf = SF_BYTES * (1 + p.nsf), stage = tile_bytes + sf;
-  float best = 0.f;
-  for (int ks = 1; ks <= 8 && ks <= kb; ks *= 2) {
-    const int share = (kb + ks - 1) / ks, red = ks > 1 ? ks * ((T + ks - 1) / ks) * BM * 4 : 0;
+  for (p.ks = 1; p.ks <= 8 && p.ks <= kb; p.ks *= 2) {
+    const int share = (kb + p.ks - 1) / p.ks, red = p.ks > 1 ? p.ks * ((T + p.ks - 1) / p.ks) * BM * 4 : 0;
     const int fixed = 1024 + red + (2 * MAX_STAGES + 3) * 8;
-    int stages = (113 * 1024 - fixed) / stage, resident = 2;   // two CTAs an SM where three stages fit into half of it
-    if (stages < 3) { stages = (224 * 1024 - fixed) / stage; resident = 1; }
-    if (stages > MAX_STAGES) stages = MAX_STAGES;
-    if (stages > share) stages = share;
-    const int ring = stages * tile_bytes > red ? stages * tile_bytes : (red + 1023) / 1024 * 1024;
-    const int smem = ring + stages * sf + fixed;
-    if (stages < 1 || smem > 227 * 1024) continue;
-    const int n = tiles * ks, rounds = (n + sms * resident - 1) / (sms * resident);
-    const float alone = 0.23f + 0.0021f * p.cols, shared = 0.2f * (n > sms ? resident : 1);
-    const float cost = rounds * (4.f + share * (alone > shared ? alone : shared));
-    if (p.ks == 0 || cost < best) {
-      best = cost;
-      p.ks = ks;
-      p.stages = stages;
-      p.ring = ring;
-      p.smem = smem;
+    for (int resident = 1; resident <= 2; ++resident) {
+      p.stages = (228 * 1024 / resident - 1024 - fixed) / stage;
+      if (p.stages > MAX_STAGES) p.stages = MAX_STAGES;
+      if (p.stages > share) p.stages = share;
+      if (p.stages < 1 || (p.stages < 3 && p.stages < share)) continue;
+      int tmem = 32;
+      while (tmem < (p.cols + 31) / 32 * 32 + p.stages * 4 * (1 + p.nsf)) tmem *= 2;
+      p.ring = p.stages * tile_bytes > red ? p.stages * tile_bytes : (red + 1023) / 1024 * 1024;
+      p.smem = p.ring + p.stages * sf + fixed;
+      // As much of an SM's shared memory as of its tensor memory (512 columns): CTAs that fit side by side, of one launch or of
+      // several streams', all get their columns.  One that waited for columns while its cluster waited for it could stop both.
+      if (p.smem < tmem * 456 - 1024) p.smem = tmem * 456 - 1024;
+      if (p.smem > 228 * 1024 / resident - 1024) continue;
+      const int n = tiles * p.ks, slots = sms * resident * (p.ks == 8 ? 7 : p.ks == 4 ? 9 : 10) / 10;
+      const int rounds = (n + slots - 1) / slots, each = n > slots ? resident : (n + sms - 1) / sms;
+      const float way = 0.0085f * (8.7f + 0.128f * p.cols);
+      float one = (way > 0.2f ? way : 0.2f) * each;
+      if (one < 0.26f) one = 0.26f;
+      p.cost = rounds * (2.f + share * one) + 2.f + 0.02f * T + (p.ks > 1 ? 2.f + 0.03f * T + (p.ks == 8 ? 1.f : 0.f) : 0.f);
+      if (best.ks == 0 || p.cost < best.cost) best = p;
     }
   }
-  return p;
+  return best;
 }
 
-inline int decode_launch(const void* codes, const void* tiles, const void* xq, long long xq_rows, int xq_cols, const uint8_t* sf,
-                         const Fp4Plan& pl, int T, int terms, int N, int kb, void* Y, long long ldy, int out_fp32, const void* bias,
-                         int bias_fp32, int* err, cudaStream_t st) {
+inline int decode_launch(const void* codes, const void* xq, long long xq_rows, int xq_cols, const Fp4Plan& pl, Fp4Params& p,
+                         cudaStream_t st) {
   CUtensorMap tmW, tmX;
-  if (make_tmap_fp4(&tmW, codes, N, static_cast<uint64_t>(kb) * BK)) return -11;
-  if (gk::make_tmap_2d(&tmX, xq, 1, xq_rows, xq_cols, xq_cols, pl.cols, BK, true)) return -12;
-  Fp4Params p;
-  p.T = T; p.Tp = pl.Tp; p.terms = terms; p.N = N; p.kb = kb; p.ks = pl.ks; p.stages = pl.stages; p.cols = pl.cols; p.ring = pl.ring;
-  p.tiles = static_cast<const uint8_t*>(tiles); p.sf = sf;
-  p.Y = Y; p.ldy = ldy; p.out_fp32 = out_fp32; p.bias = bias; p.bias_fp32 = bias_fp32; p.err = err;
-  static bool configured = false;
-  if (!configured) {
-    if (cudaFuncSetAttribute(fp4_decode_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024) != cudaSuccess) return -13;
-    configured = true;
-  }
+  if (make_tmap_fp4(&tmW, codes, p.N, static_cast<uint64_t>(p.kb) * BK)) return -11;
+  if (pl.src == ROWS16) tmX = tmW;   // not used
+  else if (gk::make_tmap_2d(&tmX, xq, 1, xq_rows, xq_cols, xq_cols, pl.cols, BK, true)) return -12;
+  p.Tp = pl.Tp; p.ks = pl.ks; p.stages = pl.stages; p.cols = pl.cols; p.ring = pl.ring;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((N + BM - 1) / BM * pl.ks, 1, 1);
+  const DecodeKernel kernel = decode_kernel(pl.src, p.T);
+  static bool configured[3][2];
+  bool& known = configured[pl.src][p.T <= 2];
+  if (!known) {
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024) != cudaSuccess) return -13;
+    known = true;
+  }
+  cfg.gridDim = dim3((p.N + BM - 1) / BM * pl.ks, 1, 1);
   cfg.blockDim = dim3(THREADS, 1, 1);
   cfg.dynamicSmemBytes = pl.smem;
   cfg.stream = st;
@@ -507,48 +628,55 @@ inline int decode_launch(const void* codes, const void* tiles, const void* xq, l
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
   attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[1].val.programmaticStreamSerializationAllowed = 1;   // behind the split kernel of the same call
+  attr[1].val.programmaticStreamSerializationAllowed = pl.src == SPLIT || gk::pdl_flag();   // behind the split of the same call
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  if (cudaLaunchKernelEx(&cfg, fp4_decode_kernel, tmW, tmX, p) != cudaSuccess) return gk::launch_status() ? gk::launch_status() : -14;
+  if (cudaLaunchKernelEx(&cfg, kernel, tmW, tmX, p) != cudaSuccess)
+    return gk::launch_status() ? gk::launch_status() : -14;
   return gk::launch_status();
 }
 
 }  // namespace gq4
 
-// Bytes of scratch (16-byte aligned) that a call wants.
+// Bytes of scratch (16-byte aligned) that a call wants; 0: none.
 GK_EXPORT long long gk_fp4_decode_scratch(int T, int terms, int Kp) {
-  const long long Tp = terms == 2 ? (T + 7) / 8 * 8 : (T + 15) / 16 * 16, cols = Tp * terms;
-  return (terms == 2 ? cols * Kp : 0) + (Kp / 128) * ((cols + 127) / 128) * 512;
+  if (terms == 1 || T <= 8) return 0;
+  const long long cols = (T + 7) / 8 * 16;
+  return cols * Kp + (Kp / 128) * ((cols + 127) / 128) * 512;
 }
 
 // y [T, N] (bf16 or fp32, row stride ldy) of activations and a weight: codes [N, Kp / 2] on a 32-byte boundary, tiles of its
-// exponents.  x: bf16 [T, K] (terms 2) or e4m3 [T, K] with exponents xs [T, K / 32] (terms 1), rows packed, 16-byte aligned;
-// K a multiple of 32, Kp of 128 and less than 128 above it.
+// exponents.  x: bf16 [T, K] (terms 2) or e4m3 [T, K] with exponents xs [T, K / 32] (terms 1), rows packed, 16-byte aligned (xs
+// 4-byte); K a multiple of 32, Kp of 128 and less than 128 above it; T up to 128.
 GK_EXPORT int gk_fp4_decode(const void* codes, const void* tiles, const void* x, const void* xs, void* scratch, void* Y,
                             long long ldy, int out_fp32, const void* bias, int bias_fp32, int T, int terms, int N, int K, int Kp,
                             int* err, void* stream) {
   using namespace gq4;
-  if ((terms != 1 && terms != 2) || T < 1 || T > 128 || N < 1 || K < 32 || K % 32 || Kp % 128 || Kp < K ||
-      Kp - K >= 128)
-    return -1;
-  if ((reinterpret_cast<uintptr_t>(codes) & 31) ||
+  if ((terms != 1 && terms != 2) || T < 1 || T > 128 || N < 1 || K < 32 || K % 32 || Kp % 128 || Kp < K || Kp - K >= 128) return -1;
+  if ((reinterpret_cast<uintptr_t>(codes) & 31) || (reinterpret_cast<uintptr_t>(xs) & 3) ||
       ((reinterpret_cast<uintptr_t>(tiles) | reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(scratch)) & 15))
     return -2;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const int kb = Kp / 128;
-  const Fp4Plan pl = plan_for(T, terms, N, kb);
+  Fp4Params p = {};
+  p.T = T; p.terms = terms; p.N = N; p.kb = Kp / 128; p.K = K;
+  p.tiles = static_cast<const uint8_t*>(tiles);
+  p.Y = Y; p.ldy = ldy; p.out_fp32 = out_fp32; p.bias = bias; p.bias_fp32 = bias_fp32; p.err = err;
+  const Fp4Plan pl = plan_for(T, terms, N, p.kb);
   if (pl.ks == 0) return -3;
-  uint8_t* ws = static_cast<uint8_t*>(scratch);
-  if (terms == 2) {
-    uint8_t* sf = ws + static_cast<long long>(pl.cols) * Kp;
-    gk::launch_k(fp4_split_kernel, dim3(grid_for(static_cast<long long>(T) * (Kp / 8))), dim3(256), 0, st,
-                 static_cast<const uint4*>(x), reinterpret_cast<uint2*>(ws), sf, T, pl.Tp, K, Kp);
-    if (int rc = gk::launch_status()) return rc;
-    return decode_launch(codes, tiles, ws, pl.cols, Kp, sf, pl, T, 2, N, kb, Y, ldy, out_fp32, bias, bias_fp32, err, st);
+  if (pl.src == ROWS8) {
+    p.sf = static_cast<const uint8_t*>(xs);
+    return decode_launch(codes, x, T, K, pl, p, st);
   }
-  gk::launch_k(fp4_tiles_kernel, dim3(grid_for(static_cast<long long>(T) * kb * 4)), dim3(256), 0, st,
-               static_cast<const uint8_t*>(xs), ws, T, K / 32, kb, pl.nsf);
+  if (pl.src == ROWS16) {
+    p.x = x;
+    return decode_launch(codes, nullptr, 0, 0, pl, p, st);
+  }
+  if (!scratch) return -2;
+  uint8_t* ws = static_cast<uint8_t*>(scratch);
+  uint8_t* sf = ws + static_cast<long long>(pl.cols) * Kp;
+  p.sf = sf;
+  gk::launch_k(fp4_split_kernel, dim3(grid_for(static_cast<long long>(T) * (Kp / 8))), dim3(256), 0, st,
+               static_cast<const uint4*>(x), reinterpret_cast<uint2*>(ws), sf, T, pl.Tp, K, Kp);
   if (int rc = gk::launch_status()) return rc;
-  return decode_launch(codes, tiles, x, T, K, ws, pl, T, 1, N, kb, Y, ldy, out_fp32, bias, bias_fp32, err, st);
+  return decode_launch(codes, ws, pl.cols, Kp, pl, p, st);
 }

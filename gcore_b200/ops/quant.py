@@ -390,17 +390,18 @@ def _fp4_decode(x2, xs, weight: Fp4Weight, bias, out_dtype):
     """Few tokens: ``x2`` [T, K] bf16, or e4m3 with exponents ``xs`` [T, K / 32] (packed, on a GPU)."""
     (T, K), N = x2.shape, weight.shape[0]
     terms = 2 if xs is None else 1
-    lib = _lib.kernels()
-    y = torch.empty(T, N, dtype=out_dtype, device=x2.device)
-    scratch = torch.empty(lib.gk_fp4_decode_scratch(T, terms, weight.padded), dtype=torch.uint8, device=x2.device)
+    lib, dev = _lib.kernels(), x2.device
+    y = torch.empty((T, N), dtype=out_dtype, device=dev)
+    need = lib.gk_fp4_decode_scratch(T, terms, weight.padded)
+    scratch = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
     if bias is not None:
         bias = (bias if bias.dtype in (torch.bfloat16, torch.float32) else bias.float()).contiguous()
-    LAUNCHES["quant"] += 2
+    LAUNCHES["quant"] += 2 if need else 1
     _lib.check(lib.gk_fp4_decode(
         weight.codes.data_ptr(), weight.tiles.data_ptr(), x2.data_ptr(), xs.data_ptr() if xs is not None else None,
-        scratch.data_ptr(), y.data_ptr(), N, out_dtype == torch.float32, bias.data_ptr() if bias is not None else None,
-        bias is not None and bias.dtype == torch.float32, T, terms, N, K, weight.padded, _lib.err_flag(x2.device).data_ptr(),
-        _lib.stream_ptr()), "fp4_decode")
+        scratch.data_ptr() if need else None, y.data_ptr(), N, out_dtype == torch.float32,
+        bias.data_ptr() if bias is not None else None, bias is not None and bias.dtype == torch.float32, T, terms, N, K,
+        weight.padded, _lib.err_flag(dev).data_ptr(), _lib.stream_ptr()), "fp4_decode")
     return y
 
 
