@@ -229,6 +229,8 @@ def _declare_kernels(lib: ctypes.CDLL):
     d("gk_fp4_dequant", [P, P, P, L, I, P])
     d("gk_mxfp8_dequant", [P, P, P, L, I, P])
     d("gk_fp4_decode_scratch", [I, I, I], L)
+    d("gk_fp4_prompt_scratch", [I, I, I], L)
+    d("gk_fp4_prompt", [P, P, P, P, P, P, L, I, P, I, I, I, I, I, I, P, P])
     d("gk_fp4_decode", [P, P, P, P, P, P, L, I, P, I, I, I, I, I, I, P, P])
     d("gk_mla_expand", [P, P, P, P, I, I, I, I, I, P])
     d("gk_mla_expand_bwd", [P, P, P, P, I, I, I, I, I, P])

@@ -475,13 +475,14 @@ fp4_decode_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant
   if (warp == 2) { tc_fence_after(); tmem_dealloc(tmem_base, tmem_cols); }
 }
 
-// bf16 rows to their terms, eight values a thread: codes [2 Tp, Kp], hi rows first, and exponents in tiles of 128 code rows.
-// Columns from K to Kp become zero.
+// bf16 rows to their terms, eight values a thread: codes [2 Tp, Kp], hi rows first, and exponents in tiles of 128 code rows x 128
+// columns, `per_kb` tiles from a K block to the next and `per_tile` from 128 rows to the next.  Columns from K to Kp become zero.
 __global__ void __launch_bounds__(256) fp4_split_kernel(const uint4* __restrict__ x, uint2* __restrict__ codes,
-                                                        uint8_t* __restrict__ sf, int T, int Tp, int K, int Kp) {
+                                                        uint8_t* __restrict__ sf, int T, int Tp, int K, int Kp, int per_kb,
+                                                        int per_tile) {
   pdl_wait();
   pdl_launch_dependents();   // behind the wait: the product takes tensor memory, which the kernel in front may still want
-  const int per = Kp / 8, live = K / 8, nsf = (2 * Tp + 127) / 128;
+  const int per = Kp / 8, live = K / 8;
   const long long units = static_cast<long long>(T) * per;   // a multiple of 16
   for (long long u0 = blockIdx.x * 256ll; u0 < units; u0 += gridDim.x * 256ll) {
     const long long u = u0 + threadIdx.x;
@@ -493,12 +494,226 @@ __global__ void __launch_bounds__(256) fp4_split_kernel(const uint4* __restrict_
       codes[u] = v.hi;
       codes[static_cast<long long>(Tp) * per + u] = v.lo;
       if ((c & 3) == 0) {
-        uint8_t* at = sf + static_cast<long long>(c >> 4) * nsf * SF_BYTES;
-        at[sf_at(t, (c >> 2) & 3)] = static_cast<uint8_t>(v.e_hi);
-        at[sf_at(Tp + t, (c >> 2) & 3)] = static_cast<uint8_t>(v.e_lo);
+        const int l = Tp + t, k4 = (c >> 2) & 3;
+        const long long kb = static_cast<long long>(c >> 4) * per_kb;
+        sf[(kb + static_cast<long long>(t >> 7) * per_tile) * SF_BYTES + sf_at(t & 127, k4)] = static_cast<uint8_t>(v.e_hi);
+        sf[(kb + static_cast<long long>(l >> 7) * per_tile) * SF_BYTES + sf_at(l & 127, k4)] = static_cast<uint8_t>(v.e_lo);
       }
     }
   }
+}
+
+// Exponents [T, K / 32] to tiles of 128 rows x 128 columns, row tile by row tile; 1 behind the last column.
+__global__ void __launch_bounds__(256) fp4_tiles_kernel(const uint8_t* __restrict__ s, uint8_t* __restrict__ sf, int T, int per,
+                                                        int kb) {
+  pdl_wait();
+  pdl_launch_dependents();
+  const long long n = static_cast<long long>(T) * kb;
+  for (long long i = blockIdx.x * 256ll + threadIdx.x; i < n; i += gridDim.x * 256ll) {
+    const int t = static_cast<int>(i / kb), k = static_cast<int>(i - static_cast<long long>(t) * kb);
+    const uint8_t* from = s + static_cast<long long>(t) * per + k * 4;
+    uint32_t w = 0;
+    if ((per & 3) == 0) {
+      w = *reinterpret_cast<const uint32_t*>(from);
+    } else {
+#pragma unroll
+      for (int b = 0; b < 4; ++b) w |= (k * 4 + b < per ? from[b] : 127u) << (8 * b);
+    }
+    *reinterpret_cast<uint32_t*>(sf + (static_cast<long long>(t >> 7) * kb + k) * SF_BYTES + sf_at(t & 127, 0)) = w;
+  }
+}
+
+// ---------------------------------------------------------------------------------------------- many tokens
+// The same product with the tokens as its rows: tiles of 128 tokens x 256 output features, one after another on each SM.  The
+// 256 columns of the sum and the exponents' columns leave no room for a second sum, so the eight epilogue warps take it to
+// registers (128 a thread) before they round and store it, and the next tile's products begin meanwhile.  TERMS = 2: both
+// terms of a bf16 row meet the weight tile in one K block, so a weight byte serves twice the operations.
+// The tensor core takes 512 cycles for a term's K block; what it needs from L2 meanwhile, 33.5 KB (TERMS = 2: 50 KB in 1024
+// cycles), is about what an SM gets.
+constexpr int PM = 128, PN = 256;
+constexpr int P_THREADS = 320;
+template <int TERMS>
+struct PromptCfg {
+  static constexpr int A_TILE = PM * BK, B_TILE = PN * BK, OPERANDS = TERMS * A_TILE + B_TILE;
+  static constexpr int SF = SF_BYTES * (TERMS + 2);
+  static constexpr int STAGES = TERMS == 1 ? 4 : 3;
+  static constexpr int SMEM = STAGES * (OPERANDS + SF) + 1024 + 256;
+  static constexpr uint32_t TX = TERMS * A_TILE + B_TILE / 2 + SF;
+};
+
+struct PromptParams {
+  int T, N, kb, mt, nt, lo_rows, band;   // mt, nt: tiles; lo_rows: code rows from a hi term to its lo term
+  const uint8_t* tiles;                  // weight exponents
+  const uint8_t* sf;                     // token exponents [code rows / 128, kb, 512]
+  void* Y;
+  long long ldy;
+  int out_fp32;
+  const void* bias;
+  int bias_fp32;
+  int* err;
+};
+
+template <int TERMS>
+__global__ void __launch_bounds__(P_THREADS, 1)
+fp4_prompt_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX, PromptParams p) {
+  using C = PromptCfg<TERMS>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sf_smem = smem + C::STAGES * C::OPERANDS;
+  uint64_t* full = reinterpret_cast<uint64_t*>(sf_smem + C::STAGES * C::SF);
+  uint64_t* empty = full + C::STAGES;
+  uint64_t* tfull = empty + C::STAGES;
+  uint64_t* tempty = tfull + 1;
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(tempty + 1);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int ntiles = p.mt * p.nt;
+  const int last_w = (p.N + BM - 1) / BM - 1;
+  constexpr int SF_COLS = 4 * (TERMS + 2);
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < C::STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
+    mbar_init(tfull, 1);
+    mbar_init(tempty, 8);
+    fence_barrier_init();
+  }
+  if (warp == 2) { tmem_alloc(tmem_holder, 512); tmem_relinquish(); }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *reinterpret_cast<volatile uint32_t*>(tmem_holder);
+  pdl_launch_dependents();   // behind the allocation, as in the kernel above
+  pdl_wait();
+
+  bool ok = true;
+  int loaded = 0;
+  if (warp == 0) {
+    int s = 0;
+    uint32_t ph = 0;
+    for (int t = blockIdx.x; t < ntiles && ok; t += gridDim.x) {
+      int mi, ni;
+      raster_tile(t, p.mt, p.nt, p.band, mi, ni);
+      for (int kb = 0; kb < p.kb; ++kb) {
+        ok = mbar_wait_warp(&empty[s], ph ^ 1, p.err, ERR_WAIT_EMPTY);
+        if (!ok) break;
+        if (lane == 0) {
+          uint8_t* a = smem + s * C::OPERANDS;
+          uint8_t* f = sf_smem + s * C::SF;
+          mbar_expect_tx(&full[s], C::TX);
+#pragma unroll
+          for (int i = 0; i < TERMS; ++i) {
+            tma_load_2d(a + i * C::A_TILE, &tmX, &full[s], kb * BK, mi * PM + i * p.lo_rows);
+            bulk_load(f + i * SF_BYTES, p.sf + (static_cast<long long>(mi + i * (p.lo_rows / PM)) * p.kb + kb) * SF_BYTES, SF_BYTES,
+                      &full[s]);
+          }
+          tma_load_2d(a + TERMS * C::A_TILE, &tmW, &full[s], kb * BK, ni * PN);
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const int w = 2 * ni + i < last_w ? 2 * ni + i : last_w;   // exponents behind the last tile meet zero codes
+            bulk_load(f + (TERMS + i) * SF_BYTES, p.tiles + (static_cast<long long>(w) * p.kb + kb) * SF_BYTES, SF_BYTES, &full[s]);
+          }
+        }
+        __syncwarp();
+        ++loaded;
+        if (++s == C::STAGES) { s = 0; ph ^= 1; }
+      }
+    }
+  } else if (warp == 1) {
+    const uint32_t go = elect_one() ? 1 : 0, idesc = mx_idesc(PM, PN, 0, 5);
+    int s = 0, n = 0;
+    uint32_t ph = 0;
+    for (int t = blockIdx.x; t < ntiles && ok; t += gridDim.x, ++n) {
+      ok = mbar_wait_warp(tempty, (n & 1) ^ 1, p.err, ERR_WAIT_TMEM_EMPTY);
+      if (!ok) break;
+      tc_fence_after();
+      for (int kb = 0; kb < p.kb; ++kb) {
+        ok = mbar_wait_warp(&full[s], ph, p.err, ERR_WAIT_FULL);
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t a = smem_u32(smem + s * C::OPERANDS), b = a + TERMS * C::A_TILE, f = smem_u32(sf_smem + s * C::SF);
+        const uint32_t sfa = tmem_base + PN + s * SF_COLS, sfb = sfa + 4 * TERMS;
+#pragma unroll
+        for (int i = 0; i < TERMS + 2; ++i) sf_to_tmem(go, sfa + 4 * i, f + SF_BYTES * i);
+#pragma unroll
+        for (int i = 0; i < TERMS; ++i)
+#pragma unroll
+          for (int k4 = 0; k4 < BK / UK; ++k4)
+            umma_mx(go, tmem_base, make_smem_desc_sw128(a + i * C::A_TILE + k4 * UK, 16, 1024),
+                    make_smem_desc_sw128(b + k4 * UK, 16, 1024), idesc + k4 * ((1u << 4) + (1u << 29)), sfa + 4 * i, sfb,
+                    (kb > 0 || i > 0 || k4 > 0) ? 1u : 0u);
+        umma_commit_if(go, &empty[s]);
+        if (kb == p.kb - 1) umma_commit_if(go, tfull);
+        if (++s == C::STAGES) { s = 0; ph ^= 1; }
+      }
+    }
+    if (!ok) {   // products under way end before the CTA gives its memory back
+      umma_commit_if(go, tfull);
+      const long long t0 = clock64();
+      while (clock64() - t0 < LAND_BUDGET_CYCLES / 10) {}
+    }
+  } else {
+    const int quad = warp & 3, half = (warp - 2) >> 2;
+    const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + half * 128;
+    int n = 0;
+    for (int t = blockIdx.x; t < ntiles; t += gridDim.x, ++n) {
+      ok = mbar_wait_warp(tfull, n & 1, p.err, ERR_WAIT_TMEM_FULL) && *reinterpret_cast<volatile int*>(p.err) == 0;
+      ok = __all_sync(0xffffffffu, ok) != 0;
+      if (!ok) break;
+      tc_fence_after();
+      uint32_t r[4][32];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) tmem_ld32(taddr + 32 * c, r[c]);
+      tmem_ld_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(tempty);
+      int mi, ni;
+      raster_tile(t, p.mt, p.nt, p.band, mi, ni);
+      const int tok = mi * PM + quad * 32 + lane, col0 = ni * PN + half * 128;
+      const bool wide = (p.ldy & 7) == 0 && (reinterpret_cast<uintptr_t>(p.Y) & 15) == 0;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const int col = col0 + c * 32 + g * 8;
+          if (tok >= p.T) continue;
+          float v[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            v[j] = __uint_as_float(r[c][g * 8 + j]);
+            if (p.bias && col + j < p.N)
+              v[j] += p.bias_fp32 ? static_cast<const float*>(p.bias)[col + j]
+                                  : __bfloat162float(static_cast<const __nv_bfloat16*>(p.bias)[col + j]);
+          }
+          const long long at = static_cast<long long>(tok) * p.ldy + col;
+          if (wide && col + 8 <= p.N) {
+            if (p.out_fp32) {
+              float4* d = reinterpret_cast<float4*>(static_cast<float*>(p.Y) + at);
+              d[0] = make_float4(v[0], v[1], v[2], v[3]);
+              d[1] = make_float4(v[4], v[5], v[6], v[7]);
+            } else {
+              *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(p.Y) + at) =
+                  make_uint4(two_bf16(v[0], v[1]), two_bf16(v[2], v[3]), two_bf16(v[4], v[5]), two_bf16(v[6], v[7]));
+            }
+          } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              if (col + j < p.N) {
+                if (p.out_fp32) static_cast<float*>(p.Y)[at + j] = v[j];
+                else static_cast<__nv_bfloat16*>(p.Y)[at + j] = __float2bfloat16(v[j]);
+              }
+          }
+        }
+      }
+      __syncwarp();
+    }
+  }
+  tc_fence_before();
+  const bool failed = __syncthreads_or(!ok);
+  if (failed && warp == 0) {
+    for (int kb = loaded > C::STAGES ? loaded - C::STAGES : 0; kb < loaded; ++kb)
+      mbar_land(&full[kb % C::STAGES], static_cast<uint32_t>(kb / C::STAGES) & 1);
+  }
+  if (warp == 2) { tc_fence_after(); tmem_dealloc(tmem_base, 512); }
 }
 
 inline unsigned grid_for(long long units) {
@@ -530,12 +745,12 @@ GK_EXPORT int gk_mxfp8_dequant(const void* q, const void* e, void* out, long lon
 
 namespace gq4 {
 
-// Codes [rows, K] (K a multiple of 128) as 128 x 128 tiles whose rows are spread to 128 bytes.
-inline int make_tmap_fp4(CUtensorMap* out, const void* base, uint64_t rows, uint64_t K) {
+// Codes [rows, K] (K a multiple of 128) as tiles of box_rows x 128 whose rows are spread to 128 bytes.
+inline int make_tmap_fp4(CUtensorMap* out, const void* base, uint64_t rows, uint64_t K, uint32_t box_rows) {
   gk::EncodeTiledFn fn = gk::get_encode_fn();
   if (!fn) return -1;
   cuuint64_t dims[2] = {K, rows}, strides[1] = {K / 2};
-  cuuint32_t box[2] = {128, 128}, estr[2] = {1, 1};
+  cuuint32_t box[2] = {128, box_rows}, estr[2] = {1, 1};
   CUresult r = CUDA_SUCCESS;
   for (int attempt = 0; attempt < 2; ++attempt) {
     r = fn(out, CU_TENSOR_MAP_DATA_TYPE_16U4_ALIGN16B, 2, const_cast<void*>(base), dims, strides, box, estr,
@@ -606,7 +821,7 @@ inline Fp4Plan plan_for(int T, int terms, int N, int kb) {
 inline int decode_launch(const void* codes, const void* xq, long long xq_rows, int xq_cols, const Fp4Plan& pl, Fp4Params& p,
                          cudaStream_t st) {
   CUtensorMap tmW, tmX;
-  if (make_tmap_fp4(&tmW, codes, p.N, static_cast<uint64_t>(p.kb) * BK)) return -11;
+  if (make_tmap_fp4(&tmW, codes, p.N, static_cast<uint64_t>(p.kb) * BK, BM)) return -11;
   if (pl.src == ROWS16) tmX = tmW;   // not used
   else if (gk::make_tmap_2d(&tmX, xq, 1, xq_rows, xq_cols, xq_cols, pl.cols, BK, true)) return -12;
   p.Tp = pl.Tp; p.ks = pl.ks; p.stages = pl.stages; p.cols = pl.cols; p.ring = pl.ring;
@@ -676,7 +891,77 @@ GK_EXPORT int gk_fp4_decode(const void* codes, const void* tiles, const void* x,
   uint8_t* sf = ws + static_cast<long long>(pl.cols) * Kp;
   p.sf = sf;
   gk::launch_k(fp4_split_kernel, dim3(grid_for(static_cast<long long>(T) * (Kp / 8))), dim3(256), 0, st,
-               static_cast<const uint4*>(x), reinterpret_cast<uint2*>(ws), sf, T, pl.Tp, K, Kp);
+               static_cast<const uint4*>(x), reinterpret_cast<uint2*>(ws), sf, T, pl.Tp, K, Kp, pl.nsf, 1);
   if (int rc = gk::launch_status()) return rc;
   return decode_launch(codes, ws, pl.cols, Kp, pl, p, st);
+}
+
+namespace gq4 {
+template <int TERMS>
+inline int prompt_launch(const void* codes, const void* xq, long long xq_rows, int xq_cols, const PromptParams& p, int Kp,
+                         cudaStream_t st) {
+  using C = PromptCfg<TERMS>;
+  CUtensorMap tmW, tmX;
+  if (make_tmap_fp4(&tmW, codes, p.N, Kp, PN)) return -11;
+  if (gk::make_tmap_2d(&tmX, xq, 1, xq_rows, xq_cols, xq_cols, PM, BK, true)) return -12;
+  static bool configured = false;
+  if (!configured) {
+    if (cudaFuncSetAttribute(fp4_prompt_kernel<TERMS>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM) != cudaSuccess) return -13;
+    configured = true;
+  }
+  const long long tiles = static_cast<long long>(p.mt) * p.nt;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(tiles < gk::sm_count() ? tiles : gk::sm_count()), 1, 1);
+  cfg.blockDim = dim3(P_THREADS, 1, 1);
+  cfg.dynamicSmemBytes = C::SMEM;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;   // behind the kernel of the same call that prepares the tokens
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (cudaLaunchKernelEx(&cfg, fp4_prompt_kernel<TERMS>, tmW, tmX, p) != cudaSuccess)
+    return gk::launch_status() ? gk::launch_status() : -14;
+  return gk::launch_status();
+}
+}  // namespace gq4
+
+// Bytes of scratch (16-byte aligned) of gk_fp4_prompt.
+GK_EXPORT long long gk_fp4_prompt_scratch(int T, int terms, int Kp) {
+  const long long rows = (T + 127) / 128 * 128ll * terms;
+  return (terms == 2 ? rows * Kp : 0) + rows / 128 * (Kp / 128) * 512;
+}
+
+// gk_fp4_decode for any number of tokens, on tiles of 128.
+GK_EXPORT int gk_fp4_prompt(const void* codes, const void* tiles, const void* x, const void* xs, void* scratch, void* Y,
+                            long long ldy, int out_fp32, const void* bias, int bias_fp32, int T, int terms, int N, int K, int Kp,
+                            int* err, void* stream) {
+  using namespace gq4;
+  if ((terms != 1 && terms != 2) || T < 1 || N < 1 || K < 32 || K % 32 || Kp % 128 || Kp < K || Kp - K >= 128 || !scratch) return -1;
+  if ((reinterpret_cast<uintptr_t>(codes) & 31) || (reinterpret_cast<uintptr_t>(xs) & 3) ||
+      ((reinterpret_cast<uintptr_t>(tiles) | reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(scratch)) & 15))
+    return -2;
+  const int kb = Kp / 128, mt = (T + PM - 1) / PM, nt = (N + PN - 1) / PN;
+  if (static_cast<long long>(mt) * nt > 0x7fffffffll) return -3;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  uint8_t* ws = static_cast<uint8_t*>(scratch);
+  PromptParams p = {};
+  p.T = T; p.N = N; p.kb = kb; p.mt = mt; p.nt = nt; p.band = gk::raster_group_m();
+  p.tiles = static_cast<const uint8_t*>(tiles);
+  p.Y = Y; p.ldy = ldy; p.out_fp32 = out_fp32; p.bias = bias; p.bias_fp32 = bias_fp32; p.err = err;
+  if (terms == 1) {
+    p.sf = ws;
+    gk::launch_k(fp4_tiles_kernel, dim3(grid_for(static_cast<long long>(T) * kb)), dim3(256), 0, st, static_cast<const uint8_t*>(xs),
+                 ws, T, K / 32, kb);
+    if (int rc = gk::launch_status()) return rc;
+    return prompt_launch<1>(codes, x, T, K, p, Kp, st);
+  }
+  const int rows = mt * PM;
+  uint8_t* sf = ws + 2ll * rows * Kp;
+  p.sf = sf;
+  p.lo_rows = rows;
+  gk::launch_k(fp4_split_kernel, dim3(grid_for(static_cast<long long>(T) * (Kp / 8))), dim3(256), 0, st,
+               static_cast<const uint4*>(x), reinterpret_cast<uint2*>(ws), sf, T, rows, K, Kp, 1, kb);
+  if (int rc = gk::launch_status()) return rc;
+  return prompt_launch<2>(codes, ws, 2ll * rows, Kp, p, Kp, st);
 }

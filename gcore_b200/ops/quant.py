@@ -383,44 +383,36 @@ def _check_fp4(what, x, weight, bias):
         raise ValueError(f"{what}: bias {tuple(bias.shape)} for {N} outputs")
 
 
-FP4_DECODE_TOKENS = 128   # most tokens of the product that streams the weight's codes
+FP4_DECODE_TOKENS = 128   # most tokens of the kernel whose tiles run over output features
 
 
-def _fp4_decode(x2, xs, weight: Fp4Weight, bias, out_dtype):
-    """Few tokens: ``x2`` [T, K] bf16, or e4m3 with exponents ``xs`` [T, K / 32] (packed, on a GPU)."""
+def _fp4_product(x2, xs, weight: Fp4Weight, bias, out_dtype):
+    """``x2`` [T, K] bf16, or e4m3 with exponents ``xs`` [T, K / 32] (packed, on a GPU), times the weight."""
     (T, K), N = x2.shape, weight.shape[0]
     terms = 2 if xs is None else 1
     lib, dev = _lib.kernels(), x2.device
     y = torch.empty((T, N), dtype=out_dtype, device=dev)
-    need = lib.gk_fp4_decode_scratch(T, terms, weight.padded)
+    if T == 0:
+        return y
+    few = T <= FP4_DECODE_TOKENS
+    need = (lib.gk_fp4_decode_scratch if few else lib.gk_fp4_prompt_scratch)(T, terms, weight.padded)
     scratch = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
     if bias is not None:
         bias = (bias if bias.dtype in (torch.bfloat16, torch.float32) else bias.float()).contiguous()
     LAUNCHES["quant"] += 2 if need else 1
-    _lib.check(lib.gk_fp4_decode(
+    _lib.check((lib.gk_fp4_decode if few else lib.gk_fp4_prompt)(
         weight.codes.data_ptr(), weight.tiles.data_ptr(), x2.data_ptr(), xs.data_ptr() if xs is not None else None,
         scratch.data_ptr() if need else None, y.data_ptr(), N, out_dtype == torch.float32,
         bias.data_ptr() if bias is not None else None, bias is not None and bias.dtype == torch.float32, T, terms, N, K,
-        weight.padded, _lib.err_flag(dev).data_ptr(), _lib.stream_ptr()), "fp4_decode")
+        weight.padded, _lib.err_flag(dev).data_ptr(), _lib.stream_ptr()), "fp4_product")
     return y
-
-
-def _fp4_product(x2, weight: Fp4Weight, bias, out_dtype):
-    """``x2`` [T, K] bf16 (packed, on a GPU) times the weight."""
-    T = x2.shape[0]
-    if T == 0:
-        return torch.empty(0, weight.shape[0], dtype=out_dtype, device=x2.device)
-    if T <= FP4_DECODE_TOKENS:
-        return _fp4_decode(x2, None, weight, bias, out_dtype)
-    from .gemm import linear_forward
-    return linear_forward(x2, weight.values(), bias, out_dtype=out_dtype)
 
 
 class _LinearFp4(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x2, weight, bias):
         ctx.weight, ctx.bias_dtype = weight, bias.dtype if bias is not None else None
-        return _fp4_product(x2, weight, bias, x2.dtype)
+        return _fp4_product(x2, None, weight, bias, x2.dtype)
 
     @staticmethod
     def backward(ctx, dy):
@@ -455,7 +447,7 @@ def linear_fp4(x: torch.Tensor, weight: Fp4Weight, bias: torch.Tensor | None = N
     if torch.is_grad_enabled() and (x.requires_grad or (bias is not None and bias.requires_grad)):
         y = _LinearFp4.apply(x2, weight, bias)
     else:
-        y = _fp4_product(x2, weight, bias, x.dtype)
+        y = _fp4_product(x2, None, weight, bias, x.dtype)
     return y if x.dim() == 2 else y.view(*x.shape[:-1], N)
 
 
@@ -481,12 +473,5 @@ def gemm_fp4(a_q: torch.Tensor, a_s: torch.Tensor, weight: Fp4Weight, bias: torc
             return gemm_fp4(a_q, a_s, weight, bias, out_dtype)
     flat = a_q.dim() == 2
     q2, s2 = _lib.packed16(a_q if flat else a_q.reshape(-1, K)), (a_s if flat else a_s.reshape(-1, K // 32)).contiguous()
-    if 1 <= q2.shape[0] <= FP4_DECODE_TOKENS:
-        y = _fp4_decode(q2, s2, weight, bias, out_dtype)
-    else:
-        x = torch.empty(q2.shape, dtype=torch.bfloat16, device=a_q.device)
-        LAUNCHES["quant"] += 1
-        _lib.check(_lib.kernels().gk_mxfp8_dequant(q2.data_ptr(), s2.data_ptr(), x.data_ptr(), q2.shape[0], K, _lib.stream_ptr()),
-                   "mxfp8_dequant")
-        y = _fp4_product(x, weight, bias, out_dtype)
+    y = _fp4_product(q2, s2, weight, bias, out_dtype)
     return y if flat else y.view(*a_q.shape[:-1], N)
