@@ -328,24 +328,22 @@ def swiglu(x: torch.Tensor, n_rows: torch.Tensor = None) -> torch.Tensor:
 
 # ------------------------------------------------------------------------------------------------ rows that end in e4m3
 def _scale_buffer(x, width, scales):
-    """Scales of rows of ``width`` values: ``fp32`` one 32-bit scale per 128, ``e8m0`` one power of two per 32."""
-    if scales == "fp32":
-        return torch.empty((*x.shape[:-1], width // 128), dtype=torch.float32, device=x.device)
-    return torch.empty((*x.shape[:-1], width // 32), dtype=torch.float8_e8m0fnu, device=x.device)
+    """Scales of ``x``'s rows, ``width`` values each: ``fp32`` one 32-bit scale per 128, ``e8m0`` one power of two per 32."""
+    n, dtype = (width // 128, torch.float32) if scales == "fp32" else (width // 32, torch.float8_e8m0fnu)
+    return torch.empty((x.shape[0], n) if x.dim() == 2 else (*x.shape[:-1], n), dtype=dtype, device=x.device)
 
 
-def _check_e4m3_rows(what, width, scales, x, *others):
-    if scales not in ("fp32", "e8m0"):
+def _check_e4m3_rows(what, width, scales, x, others=()):
+    unit = 128 if scales == "fp32" else 32 if scales == "e8m0" else 0
+    if unit == 0:
         raise ValueError(f"{what}: scales must be 'fp32' or 'e8m0', got {scales!r}")
-    if width == 0 or width % (128 if scales == "fp32" else 32):
-        raise ValueError(f"{what}: a width of {width} is not a multiple of {128 if scales == 'fp32' else 32} ({scales} scales)")
-    grads = torch.is_grad_enabled()
-    for t in (x, *others):
-        if t is not None:
-            if t.device != x.device:
-                raise ValueError(f"{what}: tensors on {x.device} and {t.device}")
-            if grads and t.requires_grad:
-                raise RuntimeError(f"{what} has no gradient: call it under torch.no_grad()")
+    if width == 0 or width % unit:
+        raise ValueError(f"{what}: a width of {width} is not a multiple of {unit} ({scales} scales)")
+    for t in others:
+        if t is not None and t.device != x.device:
+            raise ValueError(f"{what}: tensors on {x.device} and {t.device}")
+    if torch.is_grad_enabled() and (x.requires_grad or any(t is not None and t.requires_grad for t in others)):
+        raise RuntimeError(f"{what} has no gradient: call it under torch.no_grad()")
 
 
 def rmsnorm_fp8(x: torch.Tensor, w: torch.Tensor, eps: float = 1e-6, residual: torch.Tensor | None = None,
@@ -356,10 +354,10 @@ def rmsnorm_fp8(x: torch.Tensor, w: torch.Tensor, eps: float = 1e-6, residual: t
     ``quant.gemm_fp4`` reads.  The norm is rounded once, to e4m3; with ``as_rounded`` it is rounded to ``x``'s type first, so that
     ``q`` and ``s`` are those of ``quant_act_1x128(rmsnorm(...)[0])`` bit for bit.  Inference only."""
     H = x.shape[-1]
-    if w.shape != (H,) or (residual is not None and residual.shape != x.shape):
+    if w.dim() != 1 or w.shape[0] != H or (residual is not None and residual.shape != x.shape):
         raise ValueError(f"rmsnorm_fp8: x {tuple(x.shape)}, gain {tuple(w.shape)}"
                          + (f", residual {tuple(residual.shape)}" if residual is not None else ""))
-    _check_e4m3_rows("rmsnorm_fp8", H, scales, x, w, residual)
+    _check_e4m3_rows("rmsnorm_fp8", H, scales, x, (w, residual))
     bf16 = torch.bfloat16
     if not (x.dtype == bf16 and w.dtype == bf16 and (residual is None or residual.dtype == bf16) and H <= 16384
             and _lib.use_native(x)):
@@ -399,7 +397,7 @@ def swiglu_fp8(x: torch.Tensor, scales: str = "fp32", as_rounded: bool = False):
         with torch.cuda.device(x.device):
             return swiglu_fp8(x, scales, as_rounded)
     x2 = _lib.packed16(x)
-    q = torch.empty((*x.shape[:-1], F), dtype=torch.float8_e4m3fn, device=x.device)
+    q = torch.empty((x.shape[0], F) if x.dim() == 2 else (*x.shape[:-1], F), dtype=torch.float8_e4m3fn, device=x.device)
     s = _scale_buffer(x, F, scales)
     LAUNCHES["elementwise"] += 1
     _lib.check(_lib.kernels().gk_rows_quant(x2.data_ptr(), q.data_ptr(), s.data_ptr(), x2.numel() // (2 * F), F, 1,
