@@ -255,6 +255,8 @@ class InferEngineConfig(MappingMixin):
     attention_backend: str = "native"
     return_routed_experts: bool = False
     fp8_weights: bool = False
+    fp4_weights: bool = False          # dense projections served in 4 bits (what a policy trained with fp4_qat computes)
+    fp4_activations: str = "bf16"      # "bf16" | "fp8": what the 4-bit products read
     watchdog_timeout: int = 600
     model_override_args: Dict[str, Any] = field(default_factory=dict)
     override_infer_engine_config: Dict[str, Any] = field(default_factory=dict)
@@ -264,6 +266,10 @@ class InferEngineConfig(MappingMixin):
             raise ConfigError("rollout engines run with pipeline_model_parallel_size == 1")
         if not 0 < self.gpu_memory_utilization <= 1:
             raise ConfigError("gpu_memory_utilization must be in (0, 1]")
+        if self.fp4_activations not in ("bf16", "fp8"):
+            raise ConfigError("fp4_activations must be 'bf16' or 'fp8'")
+        if self.fp4_weights and self.fp8_weights:
+            raise ConfigError("projections are served in 4 bits (fp4_weights) or in block fp8 (fp8_weights), not in both")
 
 
 @dataclass

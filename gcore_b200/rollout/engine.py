@@ -171,15 +171,16 @@ class _Sched:
 
 def _count_launches() -> int:
     from ..ops import (attention, conv_norm, depth, diff_attention, gemm, head_prep, latent_attention, matrix_memory, moe, optim,
-                       rl, sandwich, scored_attention, streams, vocab, window_attention)
+                       quant, rl, sandwich, scored_attention, streams, vocab, window_attention)
     return sum(sum(m.LAUNCHES.values()) for m in (attention, conv_norm, depth, diff_attention, fused, gemm, head_prep,
-                                                  latent_attention, matrix_memory, moe, optim, rl, sandwich,
+                                                  latent_attention, matrix_memory, moe, optim, quant, rl, sandwich,
                                                   scored_attention, streams, vocab, window_attention))
 
 
 class LayerWeights:
     __slots__ = ("ln1", "qkv_w", "qkv_b", "o_w", "ln2", "fc1_w", "fc2_w", "q_ln", "k_ln", "sinks", "window", "moe",
-                 "mla", "fp8")  # fp8: {"qkv_w": (e4m3 codes, 128x128 fp32 scales), ...} when the engine serves in block fp8
+                 "mla", "fp8",  # fp8: {"qkv_w": (e4m3 codes, 128x128 fp32 scales), ...} when the engine serves in block fp8
+                 "fp4")         # fp4: {"qkv_w": Fp4Weight, ...} when it serves 4-bit weights
 
 
 class RolloutWeights:
@@ -224,7 +225,7 @@ class RolloutWeights:
         w.head = f(model.output_weight())
         for layer in model.decoder.layers:
             lw = LayerWeights()
-            lw.fp8 = None
+            lw.fp8 = lw.fp4 = None
             a = layer.self_attention
             lw.ln1 = f(layer.input_layernorm.weight)
             lw.mla = None
@@ -341,6 +342,7 @@ class InferEngine:
         self.stats = dict(decode_steps=0, prefill_tokens=0, generated_tokens=0, graph_replays=0)
         self.record_routed_experts = False
         self._peer_ar = None
+        self.fp4_activations: Optional[str] = None   # "bf16" | "fp8" when the engine serves 4-bit weights
         self.weight_scales: dict = {}  # name -> fp32 128x128 block scales when weights are held in e4m3
 
     @property
@@ -479,6 +481,8 @@ class InferEngine:
                 self._graphs.clear()
         if getattr(self, "fp8_enabled", False):
             self.quantize_weights_fp8()
+        if self.fp4_activations is not None:
+            self.quantize_weights_fp4(self.fp4_activations)
         for ent in self._mla_abs.values():
             ent[1] = True
         if self.device.type == "cuda":
@@ -492,21 +496,66 @@ class InferEngine:
         from ..ops.quant import quant_weight_128x128
         if self.plan is not None:
             raise NotImplementedError("layer-plan decoders are served in bfloat16 or float32")
-        self.fp8_enabled = True
+        self.fp8_enabled, self.fp4_activations = True, None
         for lw in self.w.layers:
-            lw.fp8 = {}
+            lw.fp8, lw.fp4 = {}, None
             for name in ("qkv_w", "o_w", "fc1_w", "fc2_w"):
                 w = getattr(lw, name)
                 if w is not None and w.dim() == 2 and w.shape[1] % 128 == 0:
                     lw.fp8[name] = quant_weight_128x128(w.to(torch.bfloat16).contiguous())
         self._graphs.clear()
 
+    # ------------------------------------------------------------------ 4-bit serving
+    def quantize_weights_fp4(self, activations: str = "bf16"):
+        """(Re)builds 4-bit copies (e2m1, one power of two per 32 columns) of every dense projection whose contraction length is a
+        multiple of 32; called after each weight hand-over like ``quantize_weights_fp8``.  ``activations="bf16"``: the products of
+        a policy trained with ``fp4_qat``, value for value; ``"fp8"``: the inputs are e4m3 with one power of two per 32 values."""
+        from ..ops.quant import Fp4Weight
+        if activations not in ("bf16", "fp8"):
+            raise ValueError(f"activations of 4-bit serving are 'bf16' or 'fp8', got {activations!r}")
+        if self.plan is not None:
+            raise NotImplementedError("layer-plan decoders are served in bfloat16 or float32")
+        self.fp8_enabled, self.fp4_activations = False, activations
+        for lw in self.w.layers:
+            lw.fp8, lw.fp4 = None, {}
+            for name in ("qkv_w", "o_w", "fc1_w", "fc2_w"):
+                w = getattr(lw, name)
+                if w is not None and w.dim() == 2 and w.shape[1] % 32 == 0:
+                    lw.fp4[name] = Fp4Weight.of(w.to(torch.bfloat16))
+        self._graphs.clear()
+
+    def _input_scales(self, h, lw: LayerWeights, name: str) -> Optional[str]:
+        """Scales of the e4m3 input that projection ``name`` takes from the kernel in front of it; None: it takes ``h``'s type."""
+        if lw.fp4 and name in lw.fp4:
+            return "e8m0" if self.fp4_activations == "fp8" else None
+        return "fp32" if lw.fp8 and name in lw.fp8 and h.dtype == torch.bfloat16 and h.is_cuda else None
+
+    def _norm_for(self, x, gamma, res, lw: LayerWeights, name: str, pending: bool = False):
+        """The norm in front of projection ``name`` and the new residual; where the projection takes e4m3 rows they come out of the
+        norm's pass (block fp8: the codes of the norm rounded to bf16, as the trainer's fp8 linear quantises it)."""
+        scales = self._input_scales(x, lw, name)
+        if scales is None or (scales == "fp32" and x.shape[-1] > 8192) or (
+                pending and self.tp > 1 and os.environ.get("GCORE_FUSED_AR_NORM", "0") == "1"):
+            return self._reduce_norm(x, gamma, res, pending)
+        if pending:
+            x = self._allreduce(x)
+        q, s, res = fused.rmsnorm_fp8(x, gamma, self.cfg.rms_norm_eps, res, scales=scales, as_rounded=scales == "fp32")
+        return (q, s), res
+
     def _lin(self, h, lw: LayerWeights, name: str, bias=None):
+        """``h`` (a tensor, or e4m3 rows and their scales) times projection ``name``."""
+        if lw.fp4 and name in lw.fp4:
+            from ..ops import quant
+            if self.fp4_activations == "bf16":
+                return quant.linear_fp4(h, lw.fp4[name], bias)
+            q, s = h if isinstance(h, tuple) else quant.quant_act_1x32(h)
+            return quant.gemm_fp4(q, s, lw.fp4[name], bias).to(self.w.embed.dtype)
         if lw.fp8 and name in lw.fp8:
             from ..ops import quant
             q, sc = lw.fp8[name]
-            aq, asc = quant.quant_act_1x128(h.to(torch.bfloat16).contiguous())
-            y = quant.gemm_fp8_blockscaled(aq, asc, q, sc, out_dtype=torch.bfloat16).to(h.dtype)
+            aq, asc = h if isinstance(h, tuple) else quant.quant_act_1x128(h.to(torch.bfloat16).contiguous())
+            y = quant.gemm_fp8_blockscaled(aq, asc, q, sc, out_dtype=torch.bfloat16)
+            y = y if isinstance(h, tuple) else y.to(h.dtype)
             return y + bias if bias is not None else y
         return linear_forward(h, getattr(lw, name), bias)
 
@@ -552,7 +601,9 @@ class InferEngine:
                 lw.moe.train()
             return y if reduce else (y, False)
         g = self._lin(h, lw, "fc1_w")
-        y = self._lin(fused.swiglu(g), lw, "fc2_w")
+        scales = self._input_scales(g, lw, "fc2_w")
+        a = fused.swiglu(g) if scales is None else fused.swiglu_fp8(g, scales=scales, as_rounded=scales == "fp32")
+        y = self._lin(a, lw, "fc2_w")
         return self._allreduce(y) if reduce else (y, self.tp > 1)
 
     def _embed(self, tokens):
@@ -579,7 +630,7 @@ class InferEngine:
             x = x.index_copy(0, embed_rows[0], embed_rows[1].to(x.dtype))
         res = None
         for li, lw in enumerate(self.w.layers):
-            h, res = fused.rmsnorm(x, lw.ln1, cfg.rms_norm_eps, res)
+            h, res = self._norm_for(x, lw.ln1, res, lw, "qkv_w")
             if lw.mla is not None:
                 packed = lw.mla.packed_ready(h, pos, cu)
                 if packed:
@@ -592,7 +643,7 @@ class InferEngine:
                     torch.cat([self._mla_cached_latent(lw.mla, c_kv), k_rope], -1))
                 a = self._allreduce(lw.mla.linear_proj(lw.mla.attend_packed(q, c_kv, k_rope, cu, max_len) if packed else
                                                        lw.mla.attend(q_nope, q_rope, c_kv, k_rope, cu, max_len)))
-                h, res = fused.rmsnorm(a, lw.ln2, cfg.rms_norm_eps, res)
+                h, res = self._norm_for(a, lw.ln2, res, lw, "fc1_w")
                 x = self._mlp(lw, h)
                 continue
             qkv = self._lin(h, lw, "qkv_w", lw.qkv_b)
@@ -603,7 +654,7 @@ class InferEngine:
             o = flash_attn_varlen(v3[:, :self.hq], v3[:, self.hq:self.hq + self.hk], v3[:, self.hq + self.hk:], cu, cu,
                                   max_len, max_len, causal=True, window=lw.window, sinks=lw.sinks)
             a = self._allreduce(self._lin(o.reshape(T, self.hq * self.D), lw, "o_w"))
-            h, res = fused.rmsnorm(a, lw.ln2, cfg.rms_norm_eps, res)
+            h, res = self._norm_for(a, lw.ln2, res, lw, "fc1_w")
             x = self._mlp(lw, h)
         last = (cu[1:] - 1).long()
         hl, _ = fused.rmsnorm(x[last], self.w.final_ln, cfg.rms_norm_eps, res[last])
@@ -670,11 +721,11 @@ class InferEngine:
                 lat_mask = p_all[None, :] < ctx[:, None]
         pending = False   # x still holds this rank's partial sums of the previous block's row-parallel projection
         for li, lw in enumerate(self.w.layers):
-            h, res = self._reduce_norm(x, lw.ln1, res, pending)
+            h, res = self._norm_for(x, lw.ln1, res, lw, "qkv_w", pending)
             if lw.mla is not None:
                 o = self._mla_decode(lw.mla, h, pos, self.k_cache[li], lat_slots, lat_idx, lat_mask,
                                      paged=(st["block_table"], ctx))
-                h, res = self._reduce_norm(lw.mla.linear_proj(o), lw.ln2, res, self.tp > 1)
+                h, res = self._norm_for(lw.mla.linear_proj(o), lw.ln2, res, lw, "fc1_w", self.tp > 1)
                 x, pending = self._mlp(lw, h, reduce=False)
                 continue
             qkv = self._lin(h, lw, "qkv_w", lw.qkv_b)
@@ -684,7 +735,7 @@ class InferEngine:
             o = paged_decode_append(qkv, pos, slots, self.k_cache[li], self.v_cache[li], st["block_table"], ctx,
                                     self.max_model_len, self.hq, self.hk, self.D, cfg.rope_theta, cfg.rotary_dim,
                                     window=lw.window, sinks=lw.sinks)
-            h, res = self._reduce_norm(self._lin(o.view(B, self.hq * self.D), lw, "o_w"), lw.ln2, res, self.tp > 1)
+            h, res = self._norm_for(self._lin(o.view(B, self.hq * self.D), lw, "o_w"), lw.ln2, res, lw, "fc1_w", self.tp > 1)
             x, pending = self._mlp(lw, h, reduce=False)
         hl, _ = self._reduce_norm(x, self.w.final_ln, res, pending)
         self._finish_decode(hl, st)

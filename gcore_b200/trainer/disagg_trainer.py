@@ -29,7 +29,9 @@ class DisaggGrpoTrainer(GrpoTrainer):
         self.policy.temperature = ie.temperature
         self.lora = bool(cfg.policy.lora.enabled)
         self.release_rollout_weights = False
-        self.serve_fp8 = False
+        if ie.fp4_weights:
+            raise NotImplementedError("fp4_weights: remote rollout engines serve the weights as they are sent")
+        self.serve_fp8 = self.serve_fp4 = False
         self.engine = None
         self.sampling = SamplingParams(temperature=ie.temperature, top_k=ie.top_k, top_p=ie.top_p, min_p=ie.min_p, repetition_penalty=ie.repetition_penalty,
                                        max_new_tokens=ie.generate_max_tokens, seed=ie.seed,

@@ -123,8 +123,10 @@ class GrpoTrainer:
         # fp8 serving: asked for by the engine config, and implied by an fp8 policy so that trainer and rollout
         # compute the same quantised products
         self.serve_fp8 = bool(getattr(ie, "fp8_weights", False) or cfg.policy.fp8)
-        if self.serve_fp8:
-            self.engine.quantize_weights_fp8()
+        self.serve_fp4, self.fp4_activations = ie.fp4_weights, ie.fp4_activations
+        if self.serve_fp4 and self.serve_fp8:
+            raise ValueError("the rollout engine serves its projections in 4 bits (fp4_weights) or in block fp8, not in both")
+        self._quantize_served_weights()
         self.engine.owns_weights = not share
         if getattr(cfg.policy, "offload_ref_model", False):
             self.policy.offload_ref_model()
@@ -323,14 +325,20 @@ class GrpoTrainer:
         else:
             from ..rollout.weight_sync import sync_weights
             sync_weights(self.policy, self.engine)
-        if self.cfg.debug.debug_update_weight and not self.lora and not self.serve_fp8:
+        if self.cfg.debug.debug_update_weight and not self.lora and not self.serve_fp8 and not self.serve_fp4:
             from ..rollout.weight_sync import verify
             bad = verify(self.policy, self.engine)
             if bad:
                 raise RuntimeError(f"rollout weights differ from the trainer's after the hand-over: {bad[:6]}")
+        # the engine's dense projections are re-quantised from the weights just handed over
+        self._quantize_served_weights()
+
+    def _quantize_served_weights(self):
+        """Low-precision copies that the rollout engine serves: e4m3 with 128x128 scales, or 4 bits with one power of two per 32."""
         if self.serve_fp8:
-            # the engine's dense projections are re-quantised (e4m3, 128x128 scales) from the weights just handed over
             self.engine.quantize_weights_fp8()
+        if self.serve_fp4:
+            self.engine.quantize_weights_fp4(self.fp4_activations)
 
     def offload_model(self):
         """Trainable weights to pinned host memory (early-swap mode of the reference's ``OffloadManager``,
