@@ -227,7 +227,6 @@ def _declare_kernels(lib: ctypes.CDLL):
     d("gk_norm_quant", [P, P, P, P, P, P, I, I, F, I, I, P])
     d("gk_rows_quant", [P, P, P, L, I, I, I, I, P])
     d("gk_fp4_dequant", [P, P, P, L, I, P])
-    d("gk_mxfp8_dequant", [P, P, P, L, I, P])
     d("gk_fp4_decode_scratch", [I, I, I], L)
     d("gk_fp4_prompt_scratch", [I, I, I], L)
     d("gk_fp4_prompt", [P, P, P, P, P, P, L, I, P, I, I, I, I, I, I, P, P])

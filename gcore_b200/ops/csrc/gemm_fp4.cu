@@ -5,6 +5,7 @@
 #include "ptx.cuh"
 #include "host_utils.h"
 #include <cuda_bf16.h>
+#include <cuda_fp4.h>
 #include <cuda_fp8.h>
 
 namespace gq4 {
@@ -14,47 +15,36 @@ using namespace gk;
 __device__ __forceinline__ float pow2_of(uint32_t e) {
   return e == 255u ? __uint_as_float(0x7fffffffu) : __uint_as_float(e << 23);
 }
-__device__ __forceinline__ float e2m1_value(uint32_t c) {
-  const uint32_t m = c & 7u;  // 0, 0.5, then (1 + m0 / 2) * 2^(e - 1)
-  const float a = m < 2u ? 0.5f * m : __uint_as_float((126u + (m >> 1)) << 23 | (m & 1u) << 22);
-  return c & 8u ? -a : a;
-}
 __device__ __forceinline__ uint32_t two_bf16(float a, float b) {
   const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
   return *reinterpret_cast<const uint32_t*>(&v);
 }
 
-// bf16 values (exact: two significant bits) of the weight, eight per thread.
+// bf16 values (exact: two significant bits) of the weight.  A CTA per tile of 128 x 128: sixteen threads a row, eight values each,
+// eight rows a thread, so that a warp writes whole lines and eight loads are under way.  Two and a half bytes a value: 6144 x
+// 4096 DEQ us (floor 9.9; one row a thread and a division each 22.7).
 __global__ void __launch_bounds__(256) fp4_dequant_kernel(const uint32_t* __restrict__ codes, const uint8_t* __restrict__ tiles,
-                                                          uint4* __restrict__ out, long long units, int per_row) {
-  for (long long u = blockIdx.x * 256ll + threadIdx.x; u < units; u += gridDim.x * 256ll) {
-    const long long row = u / per_row;
-    const int col = static_cast<int>(u - row * per_row) * 8;
-    const long long tile = (row >> 7) * (per_row >> 4) + (col >> 7);
-    const int r = static_cast<int>(row & 127);
-    const float s = pow2_of(tiles[tile * 512 + (r & 31) * 16 + (r >> 5) * 4 + ((col >> 5) & 3)]);
-    const uint32_t c = __ldcs(codes + u);
+                                                          uint4* __restrict__ out, long long N, int kb) {
+  const int k = blockIdx.x % kb;
+  const long long row0 = static_cast<long long>(blockIdx.x / kb) * 128;
+  const int c = threadIdx.x & 15, r0 = threadIdx.x >> 4;
+  const uint8_t* sf = tiles + static_cast<long long>(blockIdx.x) * 512 + (c >> 2);
+  const long long at = (row0 + r0) * kb * 16 + k * 16 + c, step = 16ll * kb * 16;   // units of eight values
+  uint32_t w[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) w[i] = row0 + r0 + 16 * i < N ? __ldcs(codes + at + i * step) : 0u;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int r = r0 + 16 * i;
+    if (row0 + r >= N) break;
+    const float s = pow2_of(sf[(r & 31) * 16 + (r >> 5) * 4]);
     uint32_t o[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) o[i] = two_bf16(e2m1_value(c >> (8 * i) & 15u) * s, e2m1_value(c >> (8 * i + 4) & 15u) * s);
-    out[u] = make_uint4(o[0], o[1], o[2], o[3]);
-  }
-}
-
-// bf16 values (exact: four significant bits) of e4m3 codes with one exponent per 32, eight per thread.
-__global__ void __launch_bounds__(256) mxfp8_dequant_kernel(const uint2* __restrict__ q, const uint8_t* __restrict__ e,
-                                                            uint4* __restrict__ out, long long units) {
-  for (long long u = blockIdx.x * 256ll + threadIdx.x; u < units; u += gridDim.x * 256ll) {
-    const float s = pow2_of(e[u >> 2]);
-    const uint2 c = q[u];
-    const uint32_t w[2] = {c.x, c.y};
-    uint32_t o[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const __half2 h = __half2(__nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(w[i >> 1] >> (16 * (i & 1))), __NV_E4M3));
-      o[i] = two_bf16(__low2float(h) * s, __high2float(h) * s);
+    for (int b = 0; b < 4; ++b) {
+      const __half2 h = __half2(__nv_cvt_fp4x2_to_halfraw2(static_cast<__nv_fp4x2_storage_t>(w[i] >> (8 * b)), __NV_E2M1));
+      o[b] = two_bf16(__low2float(h) * s, __high2float(h) * s);
     }
-    out[u] = make_uint4(o[0], o[1], o[2], o[3]);
+    out[at + i * step] = make_uint4(o[0], o[1], o[2], o[3]);
   }
 }
 
@@ -537,7 +527,8 @@ struct PromptCfg {
   static constexpr int A_TILE = PM * BK, B_TILE = PN * BK, OPERANDS = TERMS * A_TILE + B_TILE;
   static constexpr int SF = SF_BYTES * (TERMS + 2);
   static constexpr int STAGES = TERMS == 1 ? 4 : 3;
-  static constexpr int SMEM = STAGES * (OPERANDS + SF) + 1024 + 256;
+  static constexpr int PATCH = 32 * 17 * 4;   // a warp's 32 tokens x 16 features on their way to rows that are not 16-byte aligned
+  static constexpr int SMEM = STAGES * (OPERANDS + SF) + 8 * PATCH + 1024 + 256;
   static constexpr uint32_t TX = TERMS * A_TILE + B_TILE / 2 + SF;
 };
 
@@ -560,7 +551,8 @@ fp4_prompt_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sf_smem = smem + C::STAGES * C::OPERANDS;
-  uint64_t* full = reinterpret_cast<uint64_t*>(sf_smem + C::STAGES * C::SF);
+  float* patches = reinterpret_cast<float*>(sf_smem + C::STAGES * C::SF);
+  uint64_t* full = reinterpret_cast<uint64_t*>(sf_smem + C::STAGES * C::SF + 8 * C::PATCH);
   uint64_t* empty = full + C::STAGES;
   uint64_t* tfull = empty + C::STAGES;
   uint64_t* tempty = tfull + 1;
@@ -668,24 +660,20 @@ fp4_prompt_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant
       if (lane == 0) mbar_arrive(tempty);
       int mi, ni;
       raster_tile(t, p.mt, p.nt, p.band, mi, ni);
-      const int tok = mi * PM + quad * 32 + lane, col0 = ni * PN + half * 128;
-      const bool wide = (p.ldy & 7) == 0 && (reinterpret_cast<uintptr_t>(p.Y) & 15) == 0;
+      const int tok0 = mi * PM + quad * 32, tok = tok0 + lane, col0 = ni * PN + half * 128;
+      auto bias_of = [&](int col) -> float {
+        if (!p.bias || col >= p.N) return 0.f;
+        return p.bias_fp32 ? static_cast<const float*>(p.bias)[col] : __bfloat162float(static_cast<const __nv_bfloat16*>(p.bias)[col]);
+      };
+      if ((p.ldy & 7) == 0 && col0 + 128 <= p.N) {   // a lane writes its token's 128 features, 16 bytes at a time
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          const int col = col0 + c * 32 + g * 8;
-          if (tok >= p.T) continue;
+        for (int c = 0; c < 16; ++c) {
+          const int col = col0 + c * 8;
           float v[8];
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            v[j] = __uint_as_float(r[c][g * 8 + j]);
-            if (p.bias && col + j < p.N)
-              v[j] += p.bias_fp32 ? static_cast<const float*>(p.bias)[col + j]
-                                  : __bfloat162float(static_cast<const __nv_bfloat16*>(p.bias)[col + j]);
-          }
-          const long long at = static_cast<long long>(tok) * p.ldy + col;
-          if (wide && col + 8 <= p.N) {
+          for (int j = 0; j < 8; ++j) v[j] = __uint_as_float(r[c >> 2][(c & 3) * 8 + j]) + bias_of(col + j);
+          if (tok < p.T) {
+            const long long at = static_cast<long long>(tok) * p.ldy + col;
             if (p.out_fp32) {
               float4* d = reinterpret_cast<float4*>(static_cast<float*>(p.Y) + at);
               d[0] = make_float4(v[0], v[1], v[2], v[3]);
@@ -694,14 +682,26 @@ fp4_prompt_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant
               *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(p.Y) + at) =
                   make_uint4(two_bf16(v[0], v[1]), two_bf16(v[2], v[3]), two_bf16(v[4], v[5]), two_bf16(v[6], v[7]));
             }
-          } else {
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-              if (col + j < p.N) {
-                if (p.out_fp32) static_cast<float*>(p.Y)[at + j] = v[j];
-                else static_cast<__nv_bfloat16*>(p.Y)[at + j] = __float2bfloat16(v[j]);
-              }
           }
+        }
+      } else {   // rows on any boundary, the last columns: through shared memory, sixteen features of two tokens per store
+        float* patch = patches + (warp - 2) * (C::PATCH / 4);
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+          if (col0 + c * 16 >= p.N) break;
+#pragma unroll
+          for (int j = 0; j < 16; ++j) patch[lane * 17 + j] = __uint_as_float(r[c >> 1][(c & 1) * 16 + j]);
+          __syncwarp();
+          const int col = col0 + c * 16 + (lane & 15);
+          const float bias = bias_of(col);
+          for (int k = lane >> 4; k < 32 && tok0 + k < p.T; k += 2) {
+            if (col >= p.N) break;
+            const float v = patch[k * 17 + (lane & 15)] + bias;
+            const long long at = static_cast<long long>(tok0 + k) * p.ldy + col;
+            if (p.out_fp32) static_cast<float*>(p.Y)[at] = v;
+            else static_cast<__nv_bfloat16*>(p.Y)[at] = __float2bfloat16(v);
+          }
+          __syncwarp();
         }
       }
       __syncwarp();
@@ -726,20 +726,11 @@ inline unsigned grid_for(long long units) {
 // codes [N, K / 2], tiles [ceil(N / 128), K / 128, 512], out [N, K] bf16; K a multiple of 128, 16-byte aligned.
 GK_EXPORT int gk_fp4_dequant(const void* codes, const void* tiles, void* out, long long N, int K, void* stream) {
   if (N < 0 || K <= 0 || K % 128 || ((reinterpret_cast<uintptr_t>(codes) | reinterpret_cast<uintptr_t>(out)) & 15)) return -1;
-  const long long units = N * (K / 8);
-  if (units == 0) return 0;
-  gq4::fp4_dequant_kernel<<<gq4::grid_for(units), 256, 0, static_cast<cudaStream_t>(stream)>>>(
-      static_cast<const uint32_t*>(codes), static_cast<const uint8_t*>(tiles), static_cast<uint4*>(out), units, K / 8);
-  return gk::launch_status();
-}
-
-// q [T, K] e4m3, e [T, K / 32] e8m0, out [T, K] bf16; K a multiple of 32, 16-byte aligned.
-GK_EXPORT int gk_mxfp8_dequant(const void* q, const void* e, void* out, long long T, int K, void* stream) {
-  if (T < 0 || K <= 0 || K % 32 || ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) & 15)) return -1;
-  const long long units = T * (K / 8);
-  if (units == 0) return 0;
-  gq4::mxfp8_dequant_kernel<<<gq4::grid_for(units), 256, 0, static_cast<cudaStream_t>(stream)>>>(
-      static_cast<const uint2*>(q), static_cast<const uint8_t*>(e), static_cast<uint4*>(out), units);
+  const long long ctas = (N + 127) / 128 * (K / 128);
+  if (ctas == 0) return 0;
+  if (ctas > 0x7fffffffll) return -3;
+  gq4::fp4_dequant_kernel<<<static_cast<unsigned>(ctas), 256, 0, static_cast<cudaStream_t>(stream)>>>(
+      static_cast<const uint32_t*>(codes), static_cast<const uint8_t*>(tiles), static_cast<uint4*>(out), N, K / 128);
   return gk::launch_status();
 }
 
@@ -941,6 +932,7 @@ GK_EXPORT int gk_fp4_prompt(const void* codes, const void* tiles, const void* x,
   if ((reinterpret_cast<uintptr_t>(codes) & 31) || (reinterpret_cast<uintptr_t>(xs) & 3) ||
       ((reinterpret_cast<uintptr_t>(tiles) | reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(scratch)) & 15))
     return -2;
+  if (reinterpret_cast<uintptr_t>(Y) & 15) return -2;
   const int kb = Kp / 128, mt = (T + PM - 1) / PM, nt = (N + PN - 1) / PN;
   if (static_cast<long long>(mt) * nt > 0x7fffffffll) return -3;
   cudaStream_t st = static_cast<cudaStream_t>(stream);

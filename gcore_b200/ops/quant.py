@@ -391,7 +391,7 @@ def _fp4_product(x2, xs, weight: Fp4Weight, bias, out_dtype):
     (T, K), N = x2.shape, weight.shape[0]
     terms = 2 if xs is None else 1
     lib, dev = _lib.kernels(), x2.device
-    y = torch.empty((T, N), dtype=out_dtype, device=dev)
+    y = torch.empty_strided((T, N), (N, 1), dtype=out_dtype, device=dev)
     if T == 0:
         return y
     few = T <= FP4_DECODE_TOKENS
