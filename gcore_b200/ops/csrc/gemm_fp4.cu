@@ -255,15 +255,16 @@ fp4_decode_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant
     pdl_wait();
     for (int kb = 0; kb < pre; ++kb) load_tokens(kb, kb);
   }
+  // Tensor memory is taken behind the wait, and the kernel behind this one is let go when it has been: a CTA that held some while
+  // it waited for a kernel whose CTA still wanted some could stop both.
+  pdl_wait();
   if (warp == 2) { tmem_alloc(tmem_holder, tmem_cols); tmem_relinquish(); }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = *reinterpret_cast<volatile uint32_t*>(tmem_holder);
-  // not before this CTA has its tensor memory: a kernel behind it that took some and then waited for this one would stop both
   pdl_launch_dependents();
   if (p.ks > 1) cluster_arrive();   // "this CTA runs"; the wait is in front of what it is sent
-  pdl_wait();
 
   bool ok = true;
   if (warp == 0) {
@@ -471,7 +472,7 @@ __global__ void __launch_bounds__(256) fp4_split_kernel(const uint4* __restrict_
                                                         uint8_t* __restrict__ sf, int T, int Tp, int K, int Kp, int per_kb,
                                                         int per_tile) {
   pdl_wait();
-  pdl_launch_dependents();   // behind the wait: the product takes tensor memory, which the kernel in front may still want
+  pdl_launch_dependents();
   const int per = Kp / 8, live = K / 8;
   const long long units = static_cast<long long>(T) * per;   // a multiple of 16
   for (long long u0 = blockIdx.x * 256ll; u0 < units; u0 += gridDim.x * 256ll) {
@@ -568,13 +569,13 @@ fp4_prompt_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant
     mbar_init(tempty, 8);
     fence_barrier_init();
   }
+  pdl_wait();                // tensor memory is taken behind it, as in the kernel above
   if (warp == 2) { tmem_alloc(tmem_holder, 512); tmem_relinquish(); }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = *reinterpret_cast<volatile uint32_t*>(tmem_holder);
-  pdl_launch_dependents();   // behind the allocation, as in the kernel above
-  pdl_wait();
+  pdl_launch_dependents();
 
   bool ok = true;
   int loaded = 0;
@@ -761,6 +762,18 @@ inline DecodeKernel decode_kernel(int src, int T) {
   return T <= 2 ? fp4_decode_kernel<ROWS16, 1> : fp4_decode_kernel<ROWS16, 4>;
 }
 
+// Allows `kernel` all of an SM's shared memory, once per device; `done` has a bit for each.
+template <typename Kernel>
+inline int allow_shared(Kernel kernel, unsigned long long& done) {
+  int device = 0;
+  if (cudaGetDevice(&device) != cudaSuccess) return -13;
+  const unsigned long long bit = 1ull << (device & 63);
+  if (done & bit) return 0;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024) != cudaSuccess) return -13;
+  done |= bit;
+  return 0;
+}
+
 struct Fp4Plan {
   int Tp, cols, nsf, src, ks, stages, ring, smem;
   float cost;
@@ -818,12 +831,8 @@ inline int decode_launch(const void* codes, const void* xq, long long xq_rows, i
   p.Tp = pl.Tp; p.ks = pl.ks; p.stages = pl.stages; p.cols = pl.cols; p.ring = pl.ring;
   cudaLaunchConfig_t cfg = {};
   const DecodeKernel kernel = decode_kernel(pl.src, p.T);
-  static bool configured[3][2];
-  bool& known = configured[pl.src][p.T <= 2];
-  if (!known) {
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024) != cudaSuccess) return -13;
-    known = true;
-  }
+  static unsigned long long done[3][2];
+  if (int rc = allow_shared(kernel, done[pl.src][p.T <= 2])) return rc;
   cfg.gridDim = dim3((p.N + BM - 1) / BM * pl.ks, 1, 1);
   cfg.blockDim = dim3(THREADS, 1, 1);
   cfg.dynamicSmemBytes = pl.smem;
@@ -895,11 +904,8 @@ inline int prompt_launch(const void* codes, const void* xq, long long xq_rows, i
   CUtensorMap tmW, tmX;
   if (make_tmap_fp4(&tmW, codes, p.N, Kp, PN)) return -11;
   if (gk::make_tmap_2d(&tmX, xq, 1, xq_rows, xq_cols, xq_cols, PM, BK, true)) return -12;
-  static bool configured = false;
-  if (!configured) {
-    if (cudaFuncSetAttribute(fp4_prompt_kernel<TERMS>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM) != cudaSuccess) return -13;
-    configured = true;
-  }
+  static unsigned long long done = 0;
+  if (int rc = allow_shared(fp4_prompt_kernel<TERMS>, done)) return rc;
   const long long tiles = static_cast<long long>(p.mt) * p.nt;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(tiles < gk::sm_count() ? tiles : gk::sm_count()), 1, 1);

@@ -311,7 +311,8 @@ class Fp4Weight:
     """A frozen projection weight ``[N, K]`` in 4 bits, laid out once for the kernels that read it: e2m1 codes, two a byte with
     the even column in the low half, and one power of two per 32 columns.  ``codes`` uint8 [N, K / 2] and ``exponents`` (biased
     by 127; uint8 or float8_e8m0fnu, [N, K / 32]) are what ``quant_fp4_1x32`` makes and what published 4-bit checkpoints hold;
-    ``Fp4Weight.of(w)`` quantises.  K is a multiple of 32."""
+    ``Fp4Weight.of(w)`` quantises.  K is a multiple of 32.  Codes that are laid out as the kernels read them (whole tiles of 128
+    columns, packed) are kept as they are, not copied."""
 
     def __init__(self, codes: torch.Tensor, exponents: torch.Tensor):
         if codes.dtype != torch.uint8 or codes.dim() != 2:
@@ -462,6 +463,8 @@ def gemm_fp4(a_q: torch.Tensor, a_s: torch.Tensor, weight: Fp4Weight, bias: torc
     N, K = weight.shape
     if tuple(a_s.shape) != (*a_q.shape[:-1], K // 32) or a_s.device != a_q.device:
         raise ValueError(f"gemm_fp4: scales {tuple(a_s.shape)} on {a_s.device} for activations {tuple(a_q.shape)} on {a_q.device}")
+    if bias is not None and bias.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError("gemm_fp4 has no gradient: call it under torch.no_grad()")
     if out_dtype not in (torch.bfloat16, torch.float32):
         raise ValueError(f"gemm_fp4: results are bfloat16 or float32, not {out_dtype}")
     if not _lib.use_native(a_q):

@@ -151,3 +151,64 @@ def test_graphs_and_streams_side_by_side():
             y = quant.linear_fp4(xs[2], W)
     torch.cuda.synchronize()
     assert torch.equal(graphs[0][1], want[0]) and torch.equal(graphs[1][1], want[1]) and torch.equal(y, want[2])
+
+
+@pytest.mark.parametrize("T", [2, 20, 150])
+def test_tokens_that_are_not_numbers_stay_by_themselves(T):
+    """e4m3 rows with the scale of NaN, bf16 rows with an infinity: their tokens come out as NaN, the others as they were."""
+    W = weight(200, 384, seed=1)
+    x = rand(T, 384, seed=2).bfloat16()
+    want = quant.linear_fp4(x, W)
+    q, s = quant.quant_act_1x32(x)
+    want8 = quant.gemm_fp4(q, s, W)
+    x[1, 100] = float("-inf")
+    got = quant.linear_fp4(x, W)
+    s.view(torch.uint8)[1, 3] = 255
+    got8 = quant.gemm_fp4(q, s, W)
+    keep = [i for i in range(T) if i != 1]
+    assert got[1].isnan().all() and got8[1].isnan().all()
+    assert torch.equal(got[keep], want[keep]) and torch.equal(got8[keep], want8[keep])
+
+
+def test_single_rows_and_rows_in_a_batch_agree():
+    W = weight(640, 512, seed=5)
+    x = rand(12, 512, seed=3).bfloat16()
+    assert torch.equal(quant.linear_fp4(x[3], W), quant.linear_fp4(x[3:4], W)[0])
+    q, s = quant.quant_act_1x32(x[3])
+    assert torch.equal(quant.gemm_fp4(q, s, W), quant.gemm_fp4(*quant.quant_act_1x32(x[3:4]), W)[0])
+
+
+def test_a_layer_as_it_is_served_with_overlapped_launches():
+    """Norm, product, activation, product of a decode batch, launched as the rollout engine does (each kernel set up while the one
+    in front drains), thirty times over: the bits of launches one after another."""
+    from gcore_b200.ops import _lib, fused
+    up, down = weight(2048, 512, seed=1), weight(512, 1024, seed=2)
+    gain = torch.ones(512, device="cuda").bfloat16()
+    x0 = rand(24, 512, seed=3, scale=0.1).bfloat16()
+
+    def layer(x, res, eight):
+        if eight:
+            q, s, res = fused.rmsnorm_fp8(x, gain, 1e-6, res, scales="e8m0")
+            return quant.gemm_fp4(*fused.swiglu_fp8(quant.gemm_fp4(q, s, up), scales="e8m0"), down), res
+        h, res = fused.rmsnorm(x, gain, 1e-6, res)
+        return quant.linear_fp4(fused.swiglu(quant.linear_fp4(h, up)), down), res
+
+    def run(eight, T):
+        x, res, seen = x0[:T], torch.zeros_like(x0[:T]), []
+        for _ in range(30):
+            x, res = layer(x, res, eight)
+            seen += [x, res]
+        return seen
+
+    lib = _lib.kernels()
+    for T in (1, 6, 24):
+        for eight in (False, True):
+            with torch.no_grad():
+                want = run(eight, T)
+                torch.cuda.synchronize()
+                lib.gk_set_pdl(1)
+                try:
+                    got = run(eight, T)
+                finally:
+                    lib.gk_set_pdl(0)
+            assert all(torch.equal(a.nan_to_num(), b.nan_to_num()) for a, b in zip(got, want))

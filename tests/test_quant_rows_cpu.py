@@ -124,3 +124,16 @@ def test_refusals():
         quant.gemm_fp4(q, s[:1], W)
     with pytest.raises(ValueError, match="results"):
         quant.gemm_fp4(q, s, W, out_dtype=torch.float16)
+    with pytest.raises(RuntimeError, match="no gradient"):
+        quant.gemm_fp4(q, s, W, torch.ones(8, requires_grad=True))
+
+
+def test_single_rows_without_a_batch():
+    x, w = rows(1, 256, 0)[0], torch.ones(256)
+    q, s, out = fused.rmsnorm_fp8(x, w, residual=x)
+    assert q.shape == (256,) and s.shape == (2,) and out.shape == (256,)
+    q, s = fused.swiglu_fp8(x, scales="e8m0")
+    assert q.shape == (128,) and s.shape == (4,)
+    W = quant.Fp4Weight.of(rows(8, 256, 1))
+    q, s = quant.quant_act_1x32(x)
+    assert quant.linear_fp4(x, W).shape == (8,) and quant.gemm_fp4(q, s, W).shape == (8,)
