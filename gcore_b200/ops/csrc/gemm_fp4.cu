@@ -22,7 +22,7 @@ __device__ __forceinline__ uint32_t two_bf16(float a, float b) {
 
 // bf16 values (exact: two significant bits) of the weight.  A CTA per tile of 128 x 128: sixteen threads a row, eight values each,
 // eight rows a thread, so that a warp writes whole lines and eight loads are under way.  Two and a half bytes a value: 6144 x
-// 4096 DEQ us (floor 9.9; one row a thread and a division each 22.7).
+// 4096 12.3 us (floor 9.9; one row a thread and a division each 22.7).
 __global__ void __launch_bounds__(256) fp4_dequant_kernel(const uint32_t* __restrict__ codes, const uint8_t* __restrict__ tiles,
                                                           uint4* __restrict__ out, long long N, int kb) {
   const int k = blockIdx.x % kb;
@@ -528,7 +528,7 @@ struct PromptCfg {
   static constexpr int A_TILE = PM * BK, B_TILE = PN * BK, OPERANDS = TERMS * A_TILE + B_TILE;
   static constexpr int SF = SF_BYTES * (TERMS + 2);
   static constexpr int STAGES = TERMS == 1 ? 4 : 3;
-  static constexpr int PATCH = 32 * 17 * 4;   // a warp's 32 tokens x 16 features on their way to rows that are not 16-byte aligned
+  static constexpr int PATCH = 32 * 80;       // a warp's 32 tokens x 64 bytes on their way to memory, rows 80 bytes apart
   static constexpr int SMEM = STAGES * (OPERANDS + SF) + 8 * PATCH + 1024 + 256;
   static constexpr uint32_t TX = TERMS * A_TILE + B_TILE / 2 + SF;
 };
@@ -552,7 +552,7 @@ fp4_prompt_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sf_smem = smem + C::STAGES * C::OPERANDS;
-  float* patches = reinterpret_cast<float*>(sf_smem + C::STAGES * C::SF);
+  uint8_t* patches = sf_smem + C::STAGES * C::SF;
   uint64_t* full = reinterpret_cast<uint64_t*>(sf_smem + C::STAGES * C::SF + 8 * C::PATCH);
   uint64_t* empty = full + C::STAGES;
   uint64_t* tfull = empty + C::STAGES;
@@ -661,43 +661,60 @@ fp4_prompt_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant
       if (lane == 0) mbar_arrive(tempty);
       int mi, ni;
       raster_tile(t, p.mt, p.nt, p.band, mi, ni);
-      const int tok0 = mi * PM + quad * 32, tok = tok0 + lane, col0 = ni * PN + half * 128;
+      const int tok0 = mi * PM + quad * 32, col0 = ni * PN + half * 128;
       auto bias_of = [&](int col) -> float {
         if (!p.bias || col >= p.N) return 0.f;
         return p.bias_fp32 ? static_cast<const float*>(p.bias)[col] : __bfloat162float(static_cast<const __nv_bfloat16*>(p.bias)[col]);
       };
-      if ((p.ldy & 7) == 0 && col0 + 128 <= p.N) {   // a lane writes its token's 128 features, 16 bytes at a time
+      // A lane has a token's 128 features; through shared memory four lanes write 64 bytes of a token together, eight tokens an
+      // instruction (16 bytes of 32 tokens each: half-filled sectors, 787 us instead of 765 for 8192 x 28672 x 4096).
+      uint8_t* patch = patches + (warp - 2) * C::PATCH;
+      if ((p.ldy & 7) == 0 && col0 + 128 <= p.N) {
+        const int width = p.out_fp32 ? 16 : 32;   // features of a patch
 #pragma unroll
-        for (int c = 0; c < 16; ++c) {
-          const int col = col0 + c * 8;
-          float v[8];
+        for (int c = 0; c < 8; ++c) {
+          if (!p.out_fp32 && (c & 1)) continue;
+          uint4* mine = reinterpret_cast<uint4*>(patch + lane * 80);
 #pragma unroll
-          for (int j = 0; j < 8; ++j) v[j] = __uint_as_float(r[c >> 2][(c & 3) * 8 + j]) + bias_of(col + j);
-          if (tok < p.T) {
-            const long long at = static_cast<long long>(tok) * p.ldy + col;
+          for (int g = 0; g < 4; ++g) {
             if (p.out_fp32) {
-              float4* d = reinterpret_cast<float4*>(static_cast<float*>(p.Y) + at);
-              d[0] = make_float4(v[0], v[1], v[2], v[3]);
-              d[1] = make_float4(v[4], v[5], v[6], v[7]);
+              float v[4];
+#pragma unroll
+              for (int j = 0; j < 4; ++j) v[j] = __uint_as_float(r[c >> 1][(c & 1) * 16 + g * 4 + j]) + bias_of(col0 + c * 16 + g * 4 + j);
+              mine[g] = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
             } else {
-              *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(p.Y) + at) =
-                  make_uint4(two_bf16(v[0], v[1]), two_bf16(v[2], v[3]), two_bf16(v[4], v[5]), two_bf16(v[6], v[7]));
+              float v[8];
+#pragma unroll
+              for (int j = 0; j < 8; ++j) v[j] = __uint_as_float(r[c >> 1][g * 8 + j]) + bias_of(col0 + c * 16 + g * 8 + j);
+              mine[g] = make_uint4(two_bf16(v[0], v[1]), two_bf16(v[2], v[3]), two_bf16(v[4], v[5]), two_bf16(v[6], v[7]));
             }
           }
+          __syncwarp();
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const int t = k * 8 + (lane >> 2);
+            const uint4 v = *reinterpret_cast<const uint4*>(patch + t * 80 + (lane & 3) * 16);
+            if (tok0 + t < p.T) {
+              const long long at = static_cast<long long>(tok0 + t) * p.ldy + col0 + c * 16 + (lane & 3) * (width / 4);
+              if (p.out_fp32) *reinterpret_cast<uint4*>(static_cast<float*>(p.Y) + at) = v;
+              else *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(p.Y) + at) = v;
+            }
+          }
+          __syncwarp();
         }
-      } else {   // rows on any boundary, the last columns: through shared memory, sixteen features of two tokens per store
-        float* patch = patches + (warp - 2) * (C::PATCH / 4);
+      } else {   // rows on any boundary, the last columns: sixteen features of two tokens per store
+        float* rows = reinterpret_cast<float*>(patch);
 #pragma unroll
         for (int c = 0; c < 8; ++c) {
           if (col0 + c * 16 >= p.N) break;
 #pragma unroll
-          for (int j = 0; j < 16; ++j) patch[lane * 17 + j] = __uint_as_float(r[c >> 1][(c & 1) * 16 + j]);
+          for (int j = 0; j < 16; ++j) rows[lane * 17 + j] = __uint_as_float(r[c >> 1][(c & 1) * 16 + j]);
           __syncwarp();
           const int col = col0 + c * 16 + (lane & 15);
           const float bias = bias_of(col);
           for (int k = lane >> 4; k < 32 && tok0 + k < p.T; k += 2) {
             if (col >= p.N) break;
-            const float v = patch[k * 17 + (lane & 15)] + bias;
+            const float v = rows[k * 17 + (lane & 15)] + bias;
             const long long at = static_cast<long long>(tok0 + k) * p.ldy + col;
             if (p.out_fp32) static_cast<float*>(p.Y)[at] = v;
             else static_cast<__nv_bfloat16*>(p.Y)[at] = __float2bfloat16(v);
