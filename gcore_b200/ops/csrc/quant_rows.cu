@@ -43,18 +43,25 @@ __device__ __forceinline__ uint2 codes8(const float (&f)[8], float inv) {
   return make_uint2(h[0] | (h[1] << 16), h[2] | (h[3] << 16));
 }
 
+// The largest of the three sizes; NaN if one of them is.
+__device__ __forceinline__ float largest(float a, float b, float c) {
+  float d;
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
 // Eight values of a thread to codes; the 16 (SC32: 4) neighbouring lanes of its group hold the group's other values.  All lanes
 // of the warp call this; `unit` counts units of eight values over the whole matrix and picks the group's scale.
 template <bool SC32, bool AS16>
 __device__ __forceinline__ void quantise(float (&f)[8], bool live, long long unit, uint2* q, void* scales) {
   if (AS16) unpack(pack(f), f);
   if (SC32) {
-    // the comparison of bit patterns is that of sizes, with every NaN above infinity
-    uint32_t top = __float_as_uint(1e-10f);
+    float amax = 1e-10f;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(f[j]) & 0x7fffffffu);
-    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-    top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    for (int j = 0; j < 8; j += 2) amax = largest(amax, f[j], f[j + 1]);
+    amax = largest(amax, __shfl_xor_sync(0xffffffffu, amax, 1), 0.f);
+    amax = largest(amax, __shfl_xor_sync(0xffffffffu, amax, 2), 0.f);
+    const uint32_t top = __float_as_uint(amax);
     // 448 = 1.75 * 2^8: the exponent is amax's less 8, and one more where the mantissa is above 1.75
     const uint32_t e = top >= 0x7f800000u ? 255u : (top >> 23) - 8u + ((top & 0x7fffffu) > 0x600000u ? 1u : 0u);
     const float inv = __uint_as_float((254u - min(e, 253u)) << 23);
@@ -100,11 +107,16 @@ __global__ void __launch_bounds__(256) norm_quant_kernel(const Row8* __restrict_
   __shared__ float red[32];
   pdl_launch_dependents();
   const int nv = H >> 3;
+  constexpr bool WIDE = SLOTS <= 2;   // the gains stay in 32 bits where there are registers for it
   Row8 gain[SLOTS];
+  float gain32[WIDE ? SLOTS : 1][8];
 #pragma unroll
   for (int s = 0; s < SLOTS; ++s) {
     const int i = threadIdx.x + s * 256;
-    if (i < nv) gain[s] = w[i];
+    if (i < nv) {
+      gain[s] = w[i];
+      if (WIDE) unpack(gain[s], gain32[WIDE ? s : 0]);
+    }
   }
   pdl_wait();
   Row8 v[SLOTS], r[SLOTS], vn[SLOTS], rn[SLOTS];
@@ -155,9 +167,9 @@ __global__ void __launch_bounds__(256) norm_quant_kernel(const Row8* __restrict_
       if (i < nv) {
         float g[8];
         unpack(v[s], f);
-        unpack(gain[s], g);
+        if (!WIDE) unpack(gain[s], g);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) f[j] = f[j] * rstd * g[j];
+        for (int j = 0; j < 8; ++j) f[j] = f[j] * rstd * (WIDE ? gain32[WIDE ? s : 0][j] : g[j]);
       }
       quantise<SC32, AS16>(f, i < nv, at + i, q, scales);
     }
@@ -174,13 +186,23 @@ __global__ void __launch_bounds__(256) rows_quant_kernel(const Row8* __restrict_
   const long long step = static_cast<long long>(gridDim.x) * (256 * U);
   for (long long u0 = blockIdx.x * (256ll * U); u0 < units; u0 += step) {
     Row8 a[U], b[U];
+    // one division for all units of an iteration where they span two rows at most
+    const bool few = ACT && nv >= 256 * U;
+    const Index t0 = few ? static_cast<Index>(u0) / nv : 0, first = few ? static_cast<Index>(u0) - t0 * nv : 0;
 #pragma unroll
     for (int k = 0; k < U; ++k) {
       const Index u = static_cast<Index>(u0) + k * 256 + static_cast<Index>(threadIdx.x);
       if (u < units) {
         if (ACT) {
-          const Index t = u / nv;
-          const Row8* gate = in + static_cast<long long>(t) * (2 * nv) + (u - t * nv);
+          Index t = t0, i = first + k * 256 + static_cast<Index>(threadIdx.x);
+          if (!few) {
+            t = u / nv;
+            i = u - t * nv;
+          } else if (i >= nv) {
+            ++t;
+            i -= nv;
+          }
+          const Row8* gate = in + static_cast<long long>(t) * (2 * nv) + i;
           a[k] = gate[0];
           b[k] = gate[nv];
         } else {
@@ -198,7 +220,11 @@ __global__ void __launch_bounds__(256) rows_quant_kernel(const Row8* __restrict_
           float p[8];
           unpack(b[k], p);
 #pragma unroll
-          for (int j = 0; j < 8; ++j) f[j] = f[j] / (1.f + __expf(-f[j])) * p[j];
+          for (int j = 0; j < 8; ++j) {
+            // the short division: a quotient below 2^-126 is zero, which the group's floor of 1e-10 makes of it anyway
+            const float d = 1.f + __expf(-f[j]);
+            f[j] = (AS16 ? f[j] / d : __fdividef(f[j], d)) * p[j];
+          }
         }
       }
       quantise<SC32, AS16>(f, u < units, u, q, scales);
