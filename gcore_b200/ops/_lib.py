@@ -226,11 +226,10 @@ def _declare_kernels(lib: ctypes.CDLL):
     d("gk_dequant_128x128", [P, P, P, L, I, P])
     d("gk_norm_quant", [P, P, P, P, P, P, I, I, F, I, I, P])
     d("gk_rows_quant", [P, P, P, L, I, I, I, I, P])
-    d("gk_fp4_dequant", [P, P, P, L, I, P])
-    d("gk_fp4_decode_scratch", [I, I, I], L)
-    d("gk_fp4_prompt_scratch", [I, I, I], L)
-    d("gk_fp4_prompt", [P, P, P, P, P, P, L, I, P, I, I, I, I, I, I, P, P])
-    d("gk_fp4_decode", [P, P, P, P, P, P, L, I, P, I, I, I, I, I, I, P, P])
+    d("gk_fp4_dequant", [P, P, P, L, L, I, P])
+    d("gk_pad_rows16", [P, P, L, I, I, P])
+    d("gk_fp4_product_scratch", [I, I, I, I], L)
+    d("gk_fp4_product", [P, P, P, P, P, P, L, I, P, I, I, I, I, I, I, P, P])
     d("gk_mla_expand", [P, P, P, P, I, I, I, I, I, P])
     d("gk_mla_expand_bwd", [P, P, P, P, I, I, I, I, I, P])
     d("gk_latent_append", [P, L, P, P, P, P, I, I, I, F, F, I, P])

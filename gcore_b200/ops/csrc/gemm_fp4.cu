@@ -11,6 +11,11 @@
 namespace gq4 {
 using namespace gk;
 
+inline unsigned grid_for(long long units) {
+  const long long want = (units + 255) / 256, most = gk::sm_count() * 32ll;
+  return static_cast<unsigned>(want < most ? want : most);
+}
+
 // 2^(e - 127); 255 is NaN.  2^-127 and values below 2^-126 become zero (subnormals are flushed).
 __device__ __forceinline__ float pow2_of(uint32_t e) {
   return e == 255u ? __uint_as_float(0x7fffffffu) : __uint_as_float(e << 23);
@@ -24,7 +29,7 @@ __device__ __forceinline__ uint32_t two_bf16(float a, float b) {
 // eight rows a thread, so that a warp writes whole lines and eight loads are under way.  Two and a half bytes a value: 6144 x
 // 4096 12.3 us (floor 9.9; one row a thread and a division each 22.7).
 __global__ void __launch_bounds__(256) fp4_dequant_kernel(const uint32_t* __restrict__ codes, const uint8_t* __restrict__ tiles,
-                                                          uint4* __restrict__ out, long long N, int kb) {
+                                                          uint4* __restrict__ out, long long N, long long rows, int kb) {
   const int k = blockIdx.x % kb;
   const long long row0 = static_cast<long long>(blockIdx.x / kb) * 128;
   const int c = threadIdx.x & 15, r0 = threadIdx.x >> 4;
@@ -36,7 +41,7 @@ __global__ void __launch_bounds__(256) fp4_dequant_kernel(const uint32_t* __rest
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const int r = r0 + 16 * i;
-    if (row0 + r >= N) break;
+    if (row0 + r >= rows) break;
     const float s = pow2_of(sf[(r & 31) * 16 + (r >> 5) * 4]);
     uint32_t o[4];
 #pragma unroll
@@ -45,6 +50,32 @@ __global__ void __launch_bounds__(256) fp4_dequant_kernel(const uint32_t* __rest
       o[b] = two_bf16(__low2float(h) * s, __high2float(h) * s);
     }
     out[at + i * step] = make_uint4(o[0], o[1], o[2], o[3]);
+  }
+}
+
+// Rows of N 16-bit values to rows of 16-byte units, zero behind the last value: what a tensor-core operand's rows start on.  A
+// thread makes a unit out of the five words that its values lie in, whatever boundary they start on.
+__global__ void __launch_bounds__(256) pad_rows16_kernel(const uint32_t* __restrict__ src, uint4* __restrict__ dst, long long units,
+                                                         int N, int per, long long values) {
+  for (long long u = blockIdx.x * 256ll + threadIdx.x; u < units; u += gridDim.x * 256ll) {
+    const long long row = u / per;
+    const int c = static_cast<int>(u - row * per) * 8, left = N - c;   // values of the row from here on
+    const long long at = row * N + c, word = at >> 1;
+    uint32_t w[5];
+#pragma unroll
+    for (int j = 0; j < 5; ++j) {
+      const long long k = 2 * (word + j);
+      w[j] = 0;
+      if (k + 1 < values) w[j] = src[word + j];
+      else if (k < values) w[j] = reinterpret_cast<const uint16_t*>(src)[k];   // the last of an odd number
+    }
+    uint32_t o[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      o[j] = at & 1 ? __funnelshift_r(w[j], w[j + 1], 16) : w[j];
+      if (2 * j + 1 >= left) o[j] = 2 * j < left ? o[j] & 0xffffu : 0u;
+    }
+    dst[u] = make_uint4(o[0], o[1], o[2], o[3]);
   }
 }
 
@@ -78,12 +109,12 @@ enum Tokens : int {
 };
 
 struct Fp4Params {
-  int T, Tp, terms, N, kb, ks, stages, cols;   // cols: columns of the product (Tp * terms); kb: K / 128
+  int total, Tc, Tp, terms, N, kb, ks, stages, cols;   // tokens in all and per CTA; cols: columns of the product (Tp * terms)
   int K;                                       // columns that the tokens really have
   int ring;                                    // bytes of the operands' ring, or of the partial sums that use it later
   const uint8_t* tiles;                        // weight exponents
   const void* x;                               // ROWS16: rows
-  const uint8_t* sf;                           // SPLIT: exponents [kb, ceil(cols / 128), 512]; ROWS8: [T, K / 32]
+  const uint8_t* sf;                           // SPLIT: exponents [chunk, kb, ceil(cols / 128), 512]; ROWS8: [total, K / 32]
   void* Y;
   long long ldy;
   int out_fp32;
@@ -208,7 +239,8 @@ fp4_decode_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant
   const int b_bytes = p.cols * BK;                                    // a multiple of 2048
   const int stage_bytes = A_BYTES + b_bytes;
   const int sf_stage = SF_BYTES * (1 + nsf);
-  const int cs = (p.T + p.ks - 1) / p.ks;                             // token columns that a CTA of the cluster finishes
+  const int chunk = blockIdx.y, tok0 = chunk * p.Tc, T = min(p.Tc, p.total - tok0);   // this CTA's tokens
+  const int cs = (p.Tc + p.ks - 1) / p.ks;                            // token columns that a CTA of the cluster finishes
   float* part = reinterpret_cast<float*>(smem);                       // own partial sums [ks][cs][128], over the finished ring
   uint8_t* sf_smem = smem + p.ring;                                   // per stage: the weight's exponents, the tokens'
   float* red = reinterpret_cast<float*>(sf_smem + p.stages * sf_stage);   // the other CTAs' [ks][cs][128]
@@ -231,15 +263,18 @@ fp4_decode_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant
   // the gaps between the codes do not count
   const uint32_t stage_tx = A_BYTES / 2 + SF_BYTES + (SRC == ROWS16 ? 0 : b_bytes) + (SRC == SPLIT ? nsf * SF_BYTES : 0);
 
+  const uint8_t* tile_sf = p.tiles + (static_cast<long long>(tile) * p.kb + kb0) * SF_BYTES;
+  const uint8_t* token_sf = p.sf + (SRC == SPLIT ? (static_cast<long long>(chunk) * p.kb + kb0) * nsf * SF_BYTES : 0);
+  const int token_row = SRC == SPLIT ? chunk * p.cols : tok0;
   auto load_weight = [&](int s, int kb) {
     mbar_expect_tx(&full[s], stage_tx);
     tma_load_2d(smem + s * stage_bytes, &tmW, &full[s], (kb0 + kb) * BK, n0);
-    bulk_load(sf_smem + s * sf_stage, p.tiles + (static_cast<long long>(tile) * p.kb + kb0 + kb) * SF_BYTES, SF_BYTES, &full[s]);
+    bulk_load(sf_smem + s * sf_stage, tile_sf + kb * SF_BYTES, SF_BYTES, &full[s]);
   };
   auto load_tokens = [&](int s, int kb) {
-    if (SRC != ROWS16) tma_load_2d(smem + s * stage_bytes + A_BYTES, &tmX, &full[s], (kb0 + kb) * BK, 0);
+    if (SRC != ROWS16) tma_load_2d(smem + s * stage_bytes + A_BYTES, &tmX, &full[s], (kb0 + kb) * BK, token_row);
     if (SRC == SPLIT)
-      bulk_load(sf_smem + s * sf_stage + SF_BYTES, p.sf + static_cast<long long>(kb0 + kb) * nsf * SF_BYTES, SF_BYTES * nsf, &full[s]);
+      bulk_load(sf_smem + s * sf_stage + SF_BYTES, token_sf + static_cast<long long>(kb) * nsf * SF_BYTES, SF_BYTES * nsf, &full[s]);
   };
 
   int pre = 0, loaded = 0;
@@ -320,7 +355,7 @@ fp4_decode_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant
 #pragma unroll
         for (int j = 0; j < U; ++j) {
           const int t = 2 * j + t0;
-          raw[j] = kb < kblocks && t < p.T && col < p.K ? *reinterpret_cast<const uint4*>(x + static_cast<long long>(t) * p.K + col)
+          raw[j] = kb < kblocks && t < T && col < p.K ? *reinterpret_cast<const uint4*>(x + static_cast<long long>(t) * p.K + col)
                                                         : make_uint4(0, 0, 0, 0);
         }
       };
@@ -340,7 +375,7 @@ fp4_decode_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant
 #pragma unroll
         for (int j = 0; j < U; ++j) {
           const int t = 2 * j + t0, l = p.Tp + t;
-          if (t >= p.T) continue;
+          if (t >= T) continue;
           // 16-byte piece c / 2 of the row, in the order of the 128-byte swizzle
           *reinterpret_cast<uint2*>(b + t * BK + (((c >> 1) ^ (t & 7)) << 4) + (c & 1) * 8) = v[j].hi;
           *reinterpret_cast<uint2*>(b + l * BK + (((c >> 1) ^ (l & 7)) << 4) + (c & 1) * 8) = v[j].lo;
@@ -362,8 +397,8 @@ fp4_decode_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant
         for (int j = 0; j < 4; ++j) {
           const int t = lane + 32 * j;
           to[j] = 0;
-          if (t >= p.T || kb >= kblocks) continue;
-          const uint8_t* mine = p.sf + static_cast<long long>(t) * per + at;
+          if (t >= T || kb >= kblocks) continue;
+          const uint8_t* mine = p.sf + static_cast<long long>(tok0 + t) * per + at;
           if ((per & 3) == 0) {
             to[j] = *reinterpret_cast<const uint32_t*>(mine);
           } else {
@@ -383,7 +418,7 @@ fp4_decode_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant
         uint8_t* f = sf_smem + s * sf_stage + SF_BYTES;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          if (lane + 32 * j < p.T) *reinterpret_cast<uint32_t*>(f + sf_at(lane + 32 * j, 0)) = w[j];
+          if (lane + 32 * j < T) *reinterpret_cast<uint32_t*>(f + sf_at(lane + 32 * j, 0)) = w[j];
           w[j] = next[j];
         }
         fence_proxy_async();
@@ -401,24 +436,25 @@ fp4_decode_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant
     float bias = 0.f;
     if (p.bias && feat < p.N)
       bias = p.bias_fp32 ? static_cast<const float*>(p.bias)[feat] : __bfloat162float(static_cast<const __nv_bfloat16*>(p.bias)[feat]);
+    const long long y0 = tok0 * p.ldy + feat;
     auto store = [&](int tok, float v) {
-      if (p.out_fp32) static_cast<float*>(p.Y)[tok * p.ldy + feat] = v;
-      else static_cast<__nv_bfloat16*>(p.Y)[tok * p.ldy + feat] = __float2bfloat16(v);
+      if (p.out_fp32) static_cast<float*>(p.Y)[y0 + tok * p.ldy] = v;
+      else static_cast<__nv_bfloat16*>(p.Y)[y0 + tok * p.ldy] = __float2bfloat16(v);
     };
     if (ok) {
-      for (int c = half * 16; c < p.T; c += 32) {
+      for (int c = half * 16; c < T; c += 32) {
         uint32_t r[2][8], l[2][8];   // sixteen tokens a wait
         tmem_ld8(taddr + c, r[0]);
-        if (c + 8 < p.T) tmem_ld8(taddr + c + 8, r[1]);
+        if (c + 8 < T) tmem_ld8(taddr + c + 8, r[1]);
         if (p.terms == 2) {
           tmem_ld8(taddr + p.Tp + c, l[0]);
-          if (c + 8 < p.T) tmem_ld8(taddr + p.Tp + c + 8, l[1]);
+          if (c + 8 < T) tmem_ld8(taddr + p.Tp + c + 8, l[1]);
         }
         tmem_ld_wait();
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
           const int tok = c + j;
-          if (tok >= p.T) break;
+          if (tok >= T) break;
           float v = __uint_as_float(r[j >> 3][j & 7]);
           if (p.terms == 2) v += __uint_as_float(l[j >> 3][j & 7]);
           if (p.ks > 1) part[((tok & (p.ks - 1)) * cs + (tok >> ks_log)) * BM + row] = v;
@@ -443,7 +479,7 @@ fp4_decode_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant
       if (!got) mbar_land(rfull, 0);
       ok = __all_sync(0xffffffffu, ok && got && *reinterpret_cast<volatile int*>(p.err) == 0) != 0;
       if (ok && feat < p.N) {
-        for (int j = half; j * p.ks + static_cast<int>(rank) < p.T; j += 2) {
+        for (int j = half; j * p.ks + static_cast<int>(rank) < T; j += 2) {
           float v = 0.f;
           for (int r = 0; r < p.ks; ++r) v += (r == static_cast<int>(rank) ? part : red)[(r * cs + j) * BM + row];
           store(j * p.ks + rank, v + bias);
@@ -466,29 +502,34 @@ fp4_decode_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant
   if (warp == 2) { tc_fence_after(); tmem_dealloc(tmem_base, tmem_cols); }
 }
 
-// bf16 rows to their terms, eight values a thread: codes [2 Tp, Kp], hi rows first, and exponents in tiles of 128 code rows x 128
-// columns, `per_kb` tiles from a K block to the next and `per_tile` from 128 rows to the next.  Columns from K to Kp become zero.
+// bf16 rows to their terms, eight values a thread, chunk by chunk of `Tc` tokens: codes [2 Tp, Kp] of a chunk, hi rows first, and
+// exponents in tiles of 128 code rows x 128 columns, `per_chunk`, `per_kb` and `per_tile` tiles from one chunk, K block and 128
+// rows to the next.  Columns from K to Kp become zero.
+struct SplitLayout {
+  int T, Tc, Tp, K, Kp, per_chunk, per_kb, per_tile;
+};
 __global__ void __launch_bounds__(256) fp4_split_kernel(const uint4* __restrict__ x, uint2* __restrict__ codes,
-                                                        uint8_t* __restrict__ sf, int T, int Tp, int K, int Kp, int per_kb,
-                                                        int per_tile) {
+                                                        uint8_t* __restrict__ sf, SplitLayout p) {
   pdl_wait();
   pdl_launch_dependents();
-  const int per = Kp / 8, live = K / 8;
-  const long long units = static_cast<long long>(T) * per;   // a multiple of 16
+  const int per = p.Kp / 8, live = p.K / 8;
+  const long long units = static_cast<long long>(p.T) * per;   // a multiple of 16
   for (long long u0 = blockIdx.x * 256ll; u0 < units; u0 += gridDim.x * 256ll) {
     const long long u = u0 + threadIdx.x;
-    const int t = static_cast<int>(u / per), c = static_cast<int>(u - static_cast<long long>(t) * per);
+    const int tok = static_cast<int>(u / per), c = static_cast<int>(u - static_cast<long long>(tok) * per);
     uint4 raw = make_uint4(0, 0, 0, 0);
-    if (u < units && c < live) raw = x[static_cast<long long>(t) * live + c];
+    if (u < units && c < live) raw = x[static_cast<long long>(tok) * live + c];
     const Terms v = split8(raw);
     if (u < units) {
-      codes[u] = v.hi;
-      codes[static_cast<long long>(Tp) * per + u] = v.lo;
+      const int chunk = tok / p.Tc, t = tok - chunk * p.Tc, l = p.Tp + t;
+      const long long row = static_cast<long long>(chunk) * (2 * p.Tp) + t;
+      codes[row * per + c] = v.hi;
+      codes[(row + p.Tp) * per + c] = v.lo;
       if ((c & 3) == 0) {
-        const int l = Tp + t, k4 = (c >> 2) & 3;
-        const long long kb = static_cast<long long>(c >> 4) * per_kb;
-        sf[(kb + static_cast<long long>(t >> 7) * per_tile) * SF_BYTES + sf_at(t & 127, k4)] = static_cast<uint8_t>(v.e_hi);
-        sf[(kb + static_cast<long long>(l >> 7) * per_tile) * SF_BYTES + sf_at(l & 127, k4)] = static_cast<uint8_t>(v.e_lo);
+        const int k4 = (c >> 2) & 3;
+        const long long at = static_cast<long long>(chunk) * p.per_chunk + static_cast<long long>(c >> 4) * p.per_kb;
+        sf[(at + static_cast<long long>(t >> 7) * p.per_tile) * SF_BYTES + sf_at(t & 127, k4)] = static_cast<uint8_t>(v.e_hi);
+        sf[(at + static_cast<long long>(l >> 7) * p.per_tile) * SF_BYTES + sf_at(l & 127, k4)] = static_cast<uint8_t>(v.e_lo);
       }
     }
   }
@@ -662,10 +703,14 @@ fp4_prompt_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant
       int mi, ni;
       raster_tile(t, p.mt, p.nt, p.band, mi, ni);
       const int tok0 = mi * PM + quad * 32, col0 = ni * PN + half * 128;
-      auto bias_of = [&](int col) -> float {
-        if (!p.bias || col >= p.N) return 0.f;
-        return p.bias_fp32 ? static_cast<const float*>(p.bias)[col] : __bfloat162float(static_cast<const __nv_bfloat16*>(p.bias)[col]);
-      };
+      if (p.bias) {   // one branch for all values: asked for each, it took longer than the stores
+#pragma unroll
+        for (int c = 0; c < 128; ++c) {
+          const int col = col0 + c < p.N ? col0 + c : p.N - 1;
+          const float b = p.bias_fp32 ? static_cast<const float*>(p.bias)[col] : __bfloat162float(static_cast<const __nv_bfloat16*>(p.bias)[col]);
+          r[c >> 5][c & 31] = __float_as_uint(__uint_as_float(r[c >> 5][c & 31]) + b);
+        }
+      }
       // A lane has a token's 128 features; through shared memory four lanes write 64 bytes of a token together, eight tokens an
       // instruction (16 bytes of 32 tokens each: half-filled sectors, 787 us instead of 765 for 8192 x 28672 x 4096).
       uint8_t* patch = patches + (warp - 2) * C::PATCH;
@@ -680,12 +725,12 @@ fp4_prompt_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant
             if (p.out_fp32) {
               float v[4];
 #pragma unroll
-              for (int j = 0; j < 4; ++j) v[j] = __uint_as_float(r[c >> 1][(c & 1) * 16 + g * 4 + j]) + bias_of(col0 + c * 16 + g * 4 + j);
+              for (int j = 0; j < 4; ++j) v[j] = __uint_as_float(r[c >> 1][(c & 1) * 16 + g * 4 + j]);
               mine[g] = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
             } else {
               float v[8];
 #pragma unroll
-              for (int j = 0; j < 8; ++j) v[j] = __uint_as_float(r[c >> 1][g * 8 + j]) + bias_of(col0 + c * 16 + g * 8 + j);
+              for (int j = 0; j < 8; ++j) v[j] = __uint_as_float(r[c >> 1][g * 8 + j]);
               mine[g] = make_uint4(two_bf16(v[0], v[1]), two_bf16(v[2], v[3]), two_bf16(v[4], v[5]), two_bf16(v[6], v[7]));
             }
           }
@@ -702,7 +747,7 @@ fp4_prompt_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant
           }
           __syncwarp();
         }
-      } else {   // rows on any boundary, the last columns: sixteen features of two tokens per store
+      } else if (p.out_fp32) {   // rows on any boundary, the last columns: sixteen features of two tokens per store
         float* rows = reinterpret_cast<float*>(patch);
 #pragma unroll
         for (int c = 0; c < 8; ++c) {
@@ -711,13 +756,44 @@ fp4_prompt_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant
           for (int j = 0; j < 16; ++j) rows[lane * 17 + j] = __uint_as_float(r[c >> 1][(c & 1) * 16 + j]);
           __syncwarp();
           const int col = col0 + c * 16 + (lane & 15);
-          const float bias = bias_of(col);
-          for (int k = lane >> 4; k < 32 && tok0 + k < p.T; k += 2) {
-            if (col >= p.N) break;
-            const float v = rows[k * 17 + (lane & 15)] + bias;
-            const long long at = static_cast<long long>(tok0 + k) * p.ldy + col;
-            if (p.out_fp32) static_cast<float*>(p.Y)[at] = v;
-            else static_cast<__nv_bfloat16*>(p.Y)[at] = __float2bfloat16(v);
+#pragma unroll
+          for (int k = 0; k < 16; ++k) {
+            const int t = 2 * k + (lane >> 4);
+            if (tok0 + t < p.T && col < p.N)
+              static_cast<float*>(p.Y)[static_cast<long long>(tok0 + t) * p.ldy + col] = rows[t * 17 + (lane & 15)];
+          }
+          __syncwarp();
+        }
+      } else {   // in bf16 a token's 128 features at a time: 128 bytes an instruction, from the row's first or second feature as it
+                 // starts on an even or odd one (1485 x 34790 x 768: 103 us, 34816 features 70; two bytes a lane 118)
+        const int lim = p.N - col0 < 128 ? p.N - col0 : 128;
+        for (int step = 0; step < 4 && lim > 0; ++step) {
+          if (lane >> 3 == step) {
+            uint4* mine = reinterpret_cast<uint4*>(patch + (lane & 7) * 272);
+#pragma unroll
+            for (int g = 0; g < 16; ++g) {
+              float v[8];
+#pragma unroll
+              for (int j = 0; j < 8; ++j) v[j] = __uint_as_float(r[g >> 2][(g & 3) * 8 + j]);
+              mine[g] = make_uint4(two_bf16(v[0], v[1]), two_bf16(v[2], v[3]), two_bf16(v[4], v[5]), two_bf16(v[6], v[7]));
+            }
+          }
+          __syncwarp();
+          const int rows = p.T - tok0 - step * 8 < 8 ? p.T - tok0 - step * 8 : 8;
+#pragma unroll 2
+          for (int k = 0; k < rows; ++k) {
+            const long long at = static_cast<long long>(tok0 + step * 8 + k) * p.ldy + col0;
+            const int odd = static_cast<int>(at & 1);
+            uint16_t* to = static_cast<uint16_t*>(p.Y) + at;
+            const uint32_t* row = reinterpret_cast<const uint32_t*>(patch + k * 272);
+            if (odd && lane == 0) to[0] = static_cast<uint16_t>(row[0]);
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+              const int word = q * 32 + lane, e = 2 * word + odd;
+              const uint32_t v = odd ? __funnelshift_r(row[word], row[word + 1], 16) : row[word];
+              if (e + 1 < lim) *reinterpret_cast<uint32_t*>(to + e) = v;
+              else if (e < lim) to[e] = static_cast<uint16_t>(v);
+            }
           }
           __syncwarp();
         }
@@ -734,21 +810,28 @@ fp4_prompt_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant
   if (warp == 2) { tc_fence_after(); tmem_dealloc(tmem_base, 512); }
 }
 
-inline unsigned grid_for(long long units) {
-  const long long want = (units + 255) / 256, most = gk::sm_count() * 32ll;
-  return static_cast<unsigned>(want < most ? want : most);
-}
 
 }  // namespace gq4
 
-// codes [N, K / 2], tiles [ceil(N / 128), K / 128, 512], out [N, K] bf16; K a multiple of 128, 16-byte aligned.
-GK_EXPORT int gk_fp4_dequant(const void* codes, const void* tiles, void* out, long long N, int K, void* stream) {
-  if (N < 0 || K <= 0 || K % 128 || ((reinterpret_cast<uintptr_t>(codes) | reinterpret_cast<uintptr_t>(out)) & 15)) return -1;
+// codes [N, K / 2], tiles [ceil(N / 128), K / 128, 512], out [rows, K] bf16, zero from row N on; N <= rows, both in the same last
+// tile; K a multiple of 128, 16-byte aligned.
+GK_EXPORT int gk_fp4_dequant(const void* codes, const void* tiles, void* out, long long N, long long rows, int K, void* stream) {
+  if (N < 0 || rows < N || (rows + 127) / 128 != (N + 127) / 128 || K <= 0 || K % 128 || ((reinterpret_cast<uintptr_t>(codes) | reinterpret_cast<uintptr_t>(out)) & 15)) return -1;
   const long long ctas = (N + 127) / 128 * (K / 128);
   if (ctas == 0) return 0;
   if (ctas > 0x7fffffffll) return -3;
   gq4::fp4_dequant_kernel<<<static_cast<unsigned>(ctas), 256, 0, static_cast<cudaStream_t>(stream)>>>(
-      static_cast<const uint32_t*>(codes), static_cast<const uint8_t*>(tiles), static_cast<uint4*>(out), N, K / 128);
+      static_cast<const uint32_t*>(codes), static_cast<const uint8_t*>(tiles), static_cast<uint4*>(out), N, rows, K / 128);
+  return gk::launch_status();
+}
+
+// src [T, N] to dst [T, Np], zero from column N on; 16-bit values; src 4-byte and dst 16-byte aligned, Np a multiple of 8.
+GK_EXPORT int gk_pad_rows16(const void* src, void* dst, long long T, int N, int Np, void* stream) {
+  if (T < 0 || N < 1 || Np < N || Np % 8 || (reinterpret_cast<uintptr_t>(src) & 3) || (reinterpret_cast<uintptr_t>(dst) & 15)) return -1;
+  const long long units = T * (Np / 8);
+  if (units == 0) return 0;
+  gq4::pad_rows16_kernel<<<gq4::grid_for(units), 256, 0, static_cast<cudaStream_t>(stream)>>>(
+      static_cast<const uint32_t*>(src), static_cast<uint4*>(dst), units, N, Np / 8, T * N);
   return gk::launch_status();
 }
 
@@ -792,27 +875,34 @@ inline int allow_shared(Kernel kernel, unsigned long long& done) {
 }
 
 struct Fp4Plan {
-  int Tp, cols, nsf, src, ks, stages, ring, smem;
+  int T, Tc, chunks, Tp, cols, nsf, src, ks, stages, ring, smem;
   float cost;
 };
 
-// Tokens in whole columns of the product, how many CTAs share a tile's K, how deep the ring is: the cheapest by a model of what was
-// measured (B200, us).  A K block of a lone CTA takes 0.26 (the issuing warp's chain) or 0.0085 a KB of operands (60 bytes a
-// cycle, what an SM gets out of L2); two CTAs on an SM share its 0.2 of the memory's rate.  A round of CTAs costs 2, the
-// epilogue 2 + T / 50, the exchange in a cluster 2 + T / 33 and 1 more for eight CTAs, of which fewer fit into a GPC.  Chosen
-// against the others that were run, ks = 1 / 2 / 4 / 8: 1 x 4608 x 3584 12.0 / 9.5 / [9.0] / 9.8, 64 x 4608 x 3584 [14.1] / 14.6 / 21.0 /
-// 26.1, 64 x 3584 x 18944 45.7 / 31.8 / [20.6] / 27.6, 16 x 3584 x 18944 - / 25.4 / 16.7 / [15.2], 96 x 28672 x 4096 (e4m3) [23.1] / 67 / 89 /
-// 154; one or two CTAs an SM: 1 x 37888 x 3584 22.6 / [16.0], 64 x 4608 x 3584 [14.1] / 16.3.
-inline Fp4Plan plan_for(int T, int terms, int N, int kb) {
+// The decode kernel's plan: tokens per CTA (`Tc`, in whole columns of the product), how many CTAs share a tile's K, how deep the
+// ring is.  The cheapest by a model of what was measured (B200, us).  A K block of a lone CTA takes 0.26 (the issuing warp's
+// chain) or 0.0085 a KB of operands (60 bytes a cycle, what an SM gets out of L2); two CTAs on an SM share its 0.2 of the memory's
+// rate; all together get 9.5 KB a ns out of L2.  A round of CTAs costs 2 and Tc / 50 for each CTA of an SM, a launch 2, the exchange in a cluster 2 +
+// Tc / 33 and 1 more for eight CTAs, of which fewer fit into a GPC.  Chosen against the others that were run, ks = 1 / 2 / 4 / 8: 1 x
+// 4608 x 3584 12.0 / 9.5 / [9.0] / 9.8, 64 x 4608 x 3584 [14.1] / 14.6 / 21.0 / 26.1, 64 x 3584 x 18944 45.7 / 31.8 / [20.6] / 27.6, 16 x
+// 3584 x 18944 - / 25.4 / 16.7 / [15.2], 96 x 28672 x 4096 (e4m3) [23.1] / 67 / 89 / 154; one or two CTAs an SM: 1 x 37888 x 3584 22.6 /
+// [16.0], 64 x 4608 x 3584 [14.1] / 16.3.
+inline Fp4Plan decode_plan(int T, int Tc, int terms, int N, int kb) {
   Fp4Plan p = {}, best = {};
-  p.Tp = terms == 2 ? (T + 7) / 8 * 8 : (T + 15) / 16 * 16;
+  p.T = T;
+  p.Tc = Tc;
+  p.chunks = (T + Tc - 1) / Tc;
+  p.Tp = terms == 2 ? (Tc + 7) / 8 * 8 : (Tc + 15) / 16 * 16;
   p.cols = p.Tp * terms;
   p.nsf = (p.cols + 127) / 128;
   p.src = terms == 1 ? ROWS8 : T <= 8 ? ROWS16 : SPLIT;
-  const int tiles = (N + BM - 1) / BM, sms = gk::sm_count();
+  const int sms = gk::sm_count();
+  const long long tiles = (N + BM - 1ll) / BM * p.chunks;
+  if (tiles * 8 > 0x3fffffff || p.chunks > 65535) return best;
   const int tile_bytes = A_BYTES + p.cols * BK, sf = SF_BYTES * (1 + p.nsf), stage = tile_bytes + sf;
+  const float kbytes = 8.7f + 0.128f * p.cols;
   for (p.ks = 1; p.ks <= 8 && p.ks <= kb; p.ks *= 2) {
-    const int share = (kb + p.ks - 1) / p.ks, red = p.ks > 1 ? p.ks * ((T + p.ks - 1) / p.ks) * BM * 4 : 0;
+    const int share = (kb + p.ks - 1) / p.ks, red = p.ks > 1 ? p.ks * ((Tc + p.ks - 1) / p.ks) * BM * 4 : 0;
     const int fixed = 1024 + red + (2 * MAX_STAGES + 3) * 8;
     for (int resident = 1; resident <= 2; ++resident) {
       p.stages = (228 * 1024 / resident - 1024 - fixed) / stage;
@@ -827,13 +917,38 @@ inline Fp4Plan plan_for(int T, int terms, int N, int kb) {
       // several streams', all get their columns.  One that waited for columns while its cluster waited for it could stop both.
       if (p.smem < tmem * 456 - 1024) p.smem = tmem * 456 - 1024;
       if (p.smem > 228 * 1024 / resident - 1024) continue;
-      const int n = tiles * p.ks, slots = sms * resident * (p.ks == 8 ? 7 : p.ks == 4 ? 9 : 10) / 10;
+      const int n = static_cast<int>(tiles) * p.ks, slots = sms * resident * (p.ks == 8 ? 7 : p.ks == 4 ? 9 : 10) / 10;
       const int rounds = (n + slots - 1) / slots, each = n > slots ? resident : (n + sms - 1) / sms;
-      const float way = 0.0085f * (8.7f + 0.128f * p.cols);
-      float one = (way > 0.2f ? way : 0.2f) * each;
+      float one = (0.0085f * kbytes > 0.2f ? 0.0085f * kbytes : 0.2f) * each;
       if (one < 0.26f) one = 0.26f;
-      p.cost = rounds * (2.f + share * one) + 2.f + 0.02f * T + (p.ks > 1 ? 2.f + 0.03f * T + (p.ks == 8 ? 1.f : 0.f) : 0.f);
+      float loop = rounds * (2.f + 0.02f * Tc * each + share * one);
+      const float l2 = static_cast<float>(tiles) * kb * kbytes / 9500.f;
+      if (loop < l2) loop = l2;
+      p.cost = loop + 2.f + (p.ks > 1 ? 2.f + 0.03f * Tc + (p.ks == 8 ? 1.f : 0.f) : 0.f);
       if (best.ks == 0 || p.cost < best.cost) best = p;
+    }
+  }
+  return best;
+}
+
+// Which kernel, and its plan: ks = 0 for the prompt kernel.  Its tiles of 128 x 256 leave SMs without work where there are few of
+// them, and nothing divides a long K: there the decode kernel runs on chunks of the tokens.  A K block of a prompt tile takes
+// 0.45 us (0.72 of two terms), a tile 1.5 more, a launch 4.  us, prompt kernel / chunks of 128 / 64 / 32: 150 x 410 x 18912 of e4m3
+// 66 / 19.4 / [14.5] / 14.0, 936 x 417 x 1664 21.5 / 14.1 / 11.8 / [10.9], 512 x 4608 x 3584 of e4m3 17.8 / [16.6] / 17.6 / 27.4, 2048 x 1536 x
+// 1536 of e4m3 [11.7] / 13.8 / 18.4 / 25.0, 1024 x 3584 x 3584 [31.4] / 37.0 / 36.1 / 50.9.
+inline Fp4Plan plan_for(int T, int terms, int N, int kb) {
+  Fp4Plan best = {};
+  float cost = 0.f;
+  if (T > 128) {
+    const long long tiles = (T + 127ll) / 128 * ((N + 255ll) / 256), sms = gk::sm_count();
+    cost = 4.f + (tiles + sms - 1) / sms * (1.5f + kb * (terms == 1 ? 0.45f : 0.72f));
+    best.cost = cost;
+  }
+  for (int Tc = T < 128 ? T : 128; Tc >= 32 || Tc == T; Tc = Tc > 64 ? 64 : Tc > 32 ? 32 : 0) {
+    const Fp4Plan p = decode_plan(T, Tc, terms, N, kb);
+    if (p.ks > 0 && (cost == 0.f || p.cost < cost)) {
+      best = p;
+      cost = p.cost;
     }
   }
   return best;
@@ -845,12 +960,12 @@ inline int decode_launch(const void* codes, const void* xq, long long xq_rows, i
   if (make_tmap_fp4(&tmW, codes, p.N, static_cast<uint64_t>(p.kb) * BK, BM)) return -11;
   if (pl.src == ROWS16) tmX = tmW;   // not used
   else if (gk::make_tmap_2d(&tmX, xq, 1, xq_rows, xq_cols, xq_cols, pl.cols, BK, true)) return -12;
-  p.Tp = pl.Tp; p.ks = pl.ks; p.stages = pl.stages; p.cols = pl.cols; p.ring = pl.ring;
+  p.total = pl.T; p.Tc = pl.Tc; p.Tp = pl.Tp; p.ks = pl.ks; p.stages = pl.stages; p.cols = pl.cols; p.ring = pl.ring;
   cudaLaunchConfig_t cfg = {};
-  const DecodeKernel kernel = decode_kernel(pl.src, p.T);
+  const DecodeKernel kernel = decode_kernel(pl.src, pl.T);
   static unsigned long long done[3][2];
-  if (int rc = allow_shared(kernel, done[pl.src][p.T <= 2])) return rc;
-  cfg.gridDim = dim3((p.N + BM - 1) / BM * pl.ks, 1, 1);
+  if (int rc = allow_shared(kernel, done[pl.src][pl.T <= 2])) return rc;
+  cfg.gridDim = dim3((p.N + BM - 1) / BM * pl.ks, pl.chunks, 1);
   cfg.blockDim = dim3(THREADS, 1, 1);
   cfg.dynamicSmemBytes = pl.smem;
   cfg.stream = st;
@@ -869,49 +984,6 @@ inline int decode_launch(const void* codes, const void* xq, long long xq_rows, i
 }
 
 }  // namespace gq4
-
-// Bytes of scratch (16-byte aligned) that a call wants; 0: none.
-GK_EXPORT long long gk_fp4_decode_scratch(int T, int terms, int Kp) {
-  if (terms == 1 || T <= 8) return 0;
-  const long long cols = (T + 7) / 8 * 16;
-  return cols * Kp + (Kp / 128) * ((cols + 127) / 128) * 512;
-}
-
-// y [T, N] (bf16 or fp32, row stride ldy) of activations and a weight: codes [N, Kp / 2] on a 32-byte boundary, tiles of its
-// exponents.  x: bf16 [T, K] (terms 2) or e4m3 [T, K] with exponents xs [T, K / 32] (terms 1), rows packed, 16-byte aligned (xs
-// 4-byte); K a multiple of 32, Kp of 128 and less than 128 above it; T up to 128.
-GK_EXPORT int gk_fp4_decode(const void* codes, const void* tiles, const void* x, const void* xs, void* scratch, void* Y,
-                            long long ldy, int out_fp32, const void* bias, int bias_fp32, int T, int terms, int N, int K, int Kp,
-                            int* err, void* stream) {
-  using namespace gq4;
-  if ((terms != 1 && terms != 2) || T < 1 || T > 128 || N < 1 || K < 32 || K % 32 || Kp % 128 || Kp < K || Kp - K >= 128) return -1;
-  if ((reinterpret_cast<uintptr_t>(codes) & 31) || (reinterpret_cast<uintptr_t>(xs) & 3) ||
-      ((reinterpret_cast<uintptr_t>(tiles) | reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(scratch)) & 15))
-    return -2;
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
-  Fp4Params p = {};
-  p.T = T; p.terms = terms; p.N = N; p.kb = Kp / 128; p.K = K;
-  p.tiles = static_cast<const uint8_t*>(tiles);
-  p.Y = Y; p.ldy = ldy; p.out_fp32 = out_fp32; p.bias = bias; p.bias_fp32 = bias_fp32; p.err = err;
-  const Fp4Plan pl = plan_for(T, terms, N, p.kb);
-  if (pl.ks == 0) return -3;
-  if (pl.src == ROWS8) {
-    p.sf = static_cast<const uint8_t*>(xs);
-    return decode_launch(codes, x, T, K, pl, p, st);
-  }
-  if (pl.src == ROWS16) {
-    p.x = x;
-    return decode_launch(codes, nullptr, 0, 0, pl, p, st);
-  }
-  if (!scratch) return -2;
-  uint8_t* ws = static_cast<uint8_t*>(scratch);
-  uint8_t* sf = ws + static_cast<long long>(pl.cols) * Kp;
-  p.sf = sf;
-  gk::launch_k(fp4_split_kernel, dim3(grid_for(static_cast<long long>(T) * (Kp / 8))), dim3(256), 0, st,
-               static_cast<const uint4*>(x), reinterpret_cast<uint2*>(ws), sf, T, pl.Tp, K, Kp, pl.nsf, 1);
-  if (int rc = gk::launch_status()) return rc;
-  return decode_launch(codes, ws, pl.cols, Kp, pl, p, st);
-}
 
 namespace gq4 {
 template <int TERMS>
@@ -940,26 +1012,57 @@ inline int prompt_launch(const void* codes, const void* xq, long long xq_rows, i
 }
 }  // namespace gq4
 
-// Bytes of scratch (16-byte aligned) of gk_fp4_prompt.
-GK_EXPORT long long gk_fp4_prompt_scratch(int T, int terms, int Kp) {
+// Bytes of scratch (16-byte aligned) that gk_fp4_product wants; 0: none.
+GK_EXPORT long long gk_fp4_product_scratch(int T, int terms, int N, int Kp) {
+  const gq4::Fp4Plan pl = gq4::plan_for(T, terms, N, Kp / 128);
+  const long long kb = Kp / 128;
+  if (pl.ks > 0) return pl.src == gq4::SPLIT ? pl.chunks * (static_cast<long long>(pl.cols) * Kp + kb * pl.nsf * 512) : 0;
   const long long rows = (T + 127) / 128 * 128ll * terms;
-  return (terms == 2 ? rows * Kp : 0) + rows / 128 * (Kp / 128) * 512;
+  return (terms == 2 ? rows * Kp : 0) + rows / 128 * kb * 512;
 }
 
-// gk_fp4_decode for any number of tokens, on tiles of 128.
-GK_EXPORT int gk_fp4_prompt(const void* codes, const void* tiles, const void* x, const void* xs, void* scratch, void* Y,
-                            long long ldy, int out_fp32, const void* bias, int bias_fp32, int T, int terms, int N, int K, int Kp,
-                            int* err, void* stream) {
+// y [T, N] (bf16 or fp32, row stride ldy) of activations and a weight: codes [N, Kp / 2] on a 32-byte boundary, tiles of its
+// exponents.  x: bf16 [T, K] (terms 2) or e4m3 [T, K] with exponents xs [T, K / 32] (terms 1), rows packed, 16-byte aligned as
+// is Y (xs 4-byte); K a multiple of 32, Kp of 128 and less than 128 above it.
+GK_EXPORT int gk_fp4_product(const void* codes, const void* tiles, const void* x, const void* xs, void* scratch, void* Y,
+                             long long ldy, int out_fp32, const void* bias, int bias_fp32, int T, int terms, int N, int K, int Kp,
+                             int* err, void* stream) {
   using namespace gq4;
-  if ((terms != 1 && terms != 2) || T < 1 || N < 1 || K < 32 || K % 32 || Kp % 128 || Kp < K || Kp - K >= 128 || !scratch) return -1;
+  if ((terms != 1 && terms != 2) || T < 1 || N < 1 || K < 32 || K % 32 || Kp % 128 || Kp < K || Kp - K >= 128) return -1;
   if ((reinterpret_cast<uintptr_t>(codes) & 31) || (reinterpret_cast<uintptr_t>(xs) & 3) ||
-      ((reinterpret_cast<uintptr_t>(tiles) | reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(scratch)) & 15))
+      ((reinterpret_cast<uintptr_t>(tiles) | reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(scratch) |
+        reinterpret_cast<uintptr_t>(Y)) & 15))
     return -2;
-  if (reinterpret_cast<uintptr_t>(Y) & 15) return -2;
-  const int kb = Kp / 128, mt = (T + PM - 1) / PM, nt = (N + PN - 1) / PN;
-  if (static_cast<long long>(mt) * nt > 0x7fffffffll) return -3;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const int kb = Kp / 128;
+  const Fp4Plan pl = plan_for(T, terms, N, kb);
   uint8_t* ws = static_cast<uint8_t*>(scratch);
+  const unsigned split_grid = grid_for(static_cast<long long>(T) * (Kp / 8));
+  if (pl.ks > 0) {
+    Fp4Params p = {};
+    p.terms = terms; p.N = N; p.kb = kb; p.K = K;
+    p.tiles = static_cast<const uint8_t*>(tiles);
+    p.Y = Y; p.ldy = ldy; p.out_fp32 = out_fp32; p.bias = bias; p.bias_fp32 = bias_fp32; p.err = err;
+    if (pl.src == ROWS8) {
+      p.sf = static_cast<const uint8_t*>(xs);
+      return decode_launch(codes, x, T, K, pl, p, st);
+    }
+    if (pl.src == ROWS16) {
+      p.x = x;
+      return decode_launch(codes, nullptr, 0, 0, pl, p, st);
+    }
+    if (!ws) return -2;
+    const long long rows = static_cast<long long>(pl.chunks) * pl.cols;
+    uint8_t* sf = ws + rows * Kp;
+    p.sf = sf;
+    const SplitLayout lay = {T, pl.Tc, pl.Tp, K, Kp, kb * pl.nsf, pl.nsf, 1};
+    gk::launch_k(fp4_split_kernel, dim3(split_grid), dim3(256), 0, st, static_cast<const uint4*>(x), reinterpret_cast<uint2*>(ws), sf, lay);
+    if (int rc = gk::launch_status()) return rc;
+    return decode_launch(codes, ws, rows, Kp, pl, p, st);
+  }
+  if (!ws) return -2;
+  const int mt = (T + PM - 1) / PM, nt = (N + PN - 1) / PN;
+  if (static_cast<long long>(mt) * nt > 0x7fffffffll) return -3;
   PromptParams p = {};
   p.T = T; p.N = N; p.kb = kb; p.mt = mt; p.nt = nt; p.band = gk::raster_group_m();
   p.tiles = static_cast<const uint8_t*>(tiles);
@@ -975,8 +1078,8 @@ GK_EXPORT int gk_fp4_prompt(const void* codes, const void* tiles, const void* x,
   uint8_t* sf = ws + 2ll * rows * Kp;
   p.sf = sf;
   p.lo_rows = rows;
-  gk::launch_k(fp4_split_kernel, dim3(grid_for(static_cast<long long>(T) * (Kp / 8))), dim3(256), 0, st,
-               static_cast<const uint4*>(x), reinterpret_cast<uint2*>(ws), sf, T, rows, K, Kp, 1, kb);
+  const SplitLayout lay = {T, rows, rows, K, Kp, 0, 1, kb};
+  gk::launch_k(fp4_split_kernel, dim3(split_grid), dim3(256), 0, st, static_cast<const uint4*>(x), reinterpret_cast<uint2*>(ws), sf, lay);
   if (int rc = gk::launch_status()) return rc;
   return prompt_launch<2>(codes, ws, 2ll * rows, Kp, p, Kp, st);
 }

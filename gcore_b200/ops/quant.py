@@ -352,6 +352,14 @@ class Fp4Weight:
         nt, kt = self.tiles.shape[:2]
         return self.tiles.permute(0, 3, 2, 1, 4).reshape(nt * 128, kt * 4)[:self.shape[0], :self.shape[1] // 32]
 
+    def _bf16(self, rows: int) -> torch.Tensor:
+        """On a GPU: values [rows, padded columns] in bf16, zero from the last row of the weight on (rows of the same tile)."""
+        out = torch.empty(rows, self.padded, dtype=torch.bfloat16, device=self.device)
+        LAUNCHES["quant"] += 1
+        _lib.check(_lib.kernels().gk_fp4_dequant(self.codes.data_ptr(), self.tiles.data_ptr(), out.data_ptr(), self.shape[0], rows,
+                                                 self.padded, _lib.stream_ptr()), "fp4_dequant")
+        return out
+
     def values(self, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
         """The weight [N, K] in ``dtype`` (bf16 holds every value; the result may be a view of wider rows)."""
         N, K = self.shape
@@ -359,11 +367,7 @@ class Fp4Weight:
             if not _lib.is_current(self.codes):
                 with torch.cuda.device(self.device):
                     return self.values(dtype)
-            out = torch.empty(N, self.padded, dtype=dtype, device=self.device)
-            LAUNCHES["quant"] += 1
-            _lib.check(_lib.kernels().gk_fp4_dequant(self.codes.data_ptr(), self.tiles.data_ptr(), out.data_ptr(), N, self.padded,
-                                                     _lib.stream_ptr()), "fp4_dequant")
-            return out[:, :K]
+            return self._bf16(N)[:, :K]
         c = torch.stack([self.codes & 15, self.codes >> 4], dim=-1).view(N, self.padded)[:, :K].int()
         v = E2M1_VALUES.to(self.device)[c & 7] * torch.where(c >= 8, -1.0, 1.0)
         e = self.exponents.int()
@@ -384,9 +388,6 @@ def _check_fp4(what, x, weight, bias):
         raise ValueError(f"{what}: bias {tuple(bias.shape)} for {N} outputs")
 
 
-FP4_DECODE_TOKENS = 128   # most tokens of the kernel whose tiles run over output features
-
-
 def _fp4_product(x2, xs, weight: Fp4Weight, bias, out_dtype):
     """``x2`` [T, K] bf16, or e4m3 with exponents ``xs`` [T, K / 32] (packed, on a GPU), times the weight."""
     (T, K), N = x2.shape, weight.shape[0]
@@ -395,18 +396,31 @@ def _fp4_product(x2, xs, weight: Fp4Weight, bias, out_dtype):
     y = torch.empty_strided((T, N), (N, 1), dtype=out_dtype, device=dev)
     if T == 0:
         return y
-    few = T <= FP4_DECODE_TOKENS
-    need = (lib.gk_fp4_decode_scratch if few else lib.gk_fp4_prompt_scratch)(T, terms, weight.padded)
+    need = lib.gk_fp4_product_scratch(T, terms, N, weight.padded)
     scratch = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
     if bias is not None:
         bias = (bias if bias.dtype in (torch.bfloat16, torch.float32) else bias.float()).contiguous()
     LAUNCHES["quant"] += 2 if need else 1
-    _lib.check((lib.gk_fp4_decode if few else lib.gk_fp4_prompt)(
+    _lib.check(lib.gk_fp4_product(
         weight.codes.data_ptr(), weight.tiles.data_ptr(), x2.data_ptr(), xs.data_ptr() if xs is not None else None,
         scratch.data_ptr() if need else None, y.data_ptr(), N, out_dtype == torch.float32,
         bias.data_ptr() if bias is not None else None, bias is not None and bias.dtype == torch.float32, T, terms, N, K,
         weight.padded, _lib.err_flag(dev).data_ptr(), _lib.stream_ptr()), "fp4_product")
     return y
+
+
+def _fp4_dgrad(dy, weight: Fp4Weight):
+    """``dy`` [T, N] times the weight [N, K]: its bf16 values, which are exact, on the framework's GEMM.  The product reads rows of
+    ``dy`` in 16-byte units: other widths get columns of zero, and the weight as many rows of zero."""
+    from .gemm import linear_dgrad
+    (N, K), T = weight.shape, dy.shape[0]
+    wide = (N + 7) // 8 * 8
+    dy = _lib.packed16(dy)
+    if wide != N:
+        packed, dy = dy, torch.empty(T, wide, dtype=dy.dtype, device=dy.device)
+        LAUNCHES["quant"] += 1
+        _lib.check(_lib.kernels().gk_pad_rows16(packed.data_ptr(), dy.data_ptr(), T, N, wide, _lib.stream_ptr()), "pad_rows16")
+    return linear_dgrad(dy, weight._bf16(wide)[:, :K])
 
 
 class _LinearFp4(torch.autograd.Function):
@@ -419,15 +433,11 @@ class _LinearFp4(torch.autograd.Function):
     def backward(ctx, dy):
         dx = db = None
         if ctx.needs_input_grad[0]:
-            from .gemm import linear_dgrad
             N, K = ctx.weight.shape
-            w = ctx.weight.values()
-            pad = -N % 8   # the product reads rows in 16-byte units
-            if pad:
-                dy8, w = torch.nn.functional.pad(dy, (0, pad)), torch.nn.functional.pad(w, (0, 0, 0, pad))
+            if dy.shape[0] == 0:
+                dx = dy.new_empty(0, K)
             else:
-                dy8 = _lib.packed16(dy)
-            dx = linear_dgrad(dy8, w) if dy.shape[0] else dy.new_empty(0, K)
+                dx = _fp4_dgrad(dy.to(torch.bfloat16), ctx.weight)
         if ctx.needs_input_grad[2]:
             db = dy.float().sum(0).to(ctx.bias_dtype)
         return dx, None, db

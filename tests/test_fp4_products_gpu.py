@@ -32,7 +32,9 @@ def bound(x, w, y, dtype):
 
 
 SIZES = [(1, 128, 32), (1, 300, 3584), (3, 1, 64), (8, 129, 256), (13, 4608, 3584), (16, 513, 1184), (33, 3584, 4128), (64, 896, 18944),
-         (100, 1027, 512), (128, 256, 1536), (129, 640, 1024), (257, 2293, 1056), (1000, 384, 2048)]
+         (100, 1027, 512), (128, 256, 1536), (129, 640, 1024), (257, 2293, 1056), (1000, 384, 2048),
+         # few tiles: chunks of the tokens, with and without a divided sum; many tiles of the widths that are not whole units
+         (150, 130, 4608), (300, 70, 2080), (129, 129, 128), (641, 513, 672), (1300, 6401, 256), (700, 12802, 160), (520, 9999, 384)]
 
 
 @pytest.mark.parametrize("T,N,K", SIZES)
@@ -106,7 +108,7 @@ def test_row_strides_batches_and_empty():
     assert quant.gemm_fp4(q, s, W).shape == (0, 256)
 
 
-@pytest.mark.parametrize("T,N,K", [(1, 64, 96), (40, 257, 320), (300, 1024, 512), (513, 130, 1152)])
+@pytest.mark.parametrize("T,N,K", [(1, 64, 96), (40, 257, 320), (300, 1024, 512), (513, 130, 1152), (257, 1, 64), (131, 903, 256)])
 def test_gradient(T, N, K):
     W = weight(N, K, seed=N)
     w = W.values(torch.float32).double()
