@@ -485,6 +485,6 @@ def gemm_fp4(a_q: torch.Tensor, a_s: torch.Tensor, weight: Fp4Weight, bias: torc
         with torch.cuda.device(a_q.device):
             return gemm_fp4(a_q, a_s, weight, bias, out_dtype)
     flat = a_q.dim() == 2
-    q2, s2 = _lib.packed16(a_q if flat else a_q.reshape(-1, K)), (a_s if flat else a_s.reshape(-1, K // 32)).contiguous()
+    q2, s2 = _lib.packed16(a_q if flat else a_q.reshape(-1, K)), _lib.packed16(a_s if flat else a_s.reshape(-1, K // 32))
     y = _fp4_product(q2, s2, weight, bias, out_dtype)
     return y if flat else y.view(*a_q.shape[:-1], N)

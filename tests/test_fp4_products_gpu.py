@@ -106,6 +106,22 @@ def test_row_strides_batches_and_empty():
     assert quant.linear_fp4(x[:0, :512], W).shape == (0, 256)
     q, s = quant.quant_act_1x32(x[:0, :512])
     assert quant.gemm_fp4(q, s, W).shape == (0, 256)
+    # rows of three exponents that start on any byte, scales and codes of wider buffers
+    V = weight(40, 96, seed=3)
+    q, s = quant.quant_act_1x32(x[:, :96])
+    want = quant.gemm_fp4(q, s, V)
+    for i in range(1, 5):
+        assert torch.equal(quant.gemm_fp4(q[i:], s[i:], V), want[i:])
+    wide_q, wide_s = torch.zeros(6, 200, device="cuda").to(torch.float8_e4m3fn), torch.empty(6, 7, dtype=torch.uint8, device="cuda")
+    wide_q[:, 5:101], wide_s[:, 2:5] = q, s.view(torch.uint8)
+    assert torch.equal(quant.gemm_fp4(wide_q[:, 5:101], wide_s.view(torch.float8_e8m0fnu)[:, 2:5], V), want)
+    # a weight cut out of a larger one
+    big = quant.Fp4Weight.of(rand(80, 512, seed=9).bfloat16())
+    part = quant.Fp4Weight(big.codes[3:44, 16:64], big.exponents[3:44, 1:4])
+    assert torch.equal(part.values(), big.values()[3:44, 32:128])
+    y = x[:, :96].double() @ part.values().double().t()
+    assert ((quant.linear_fp4(x[:, :96], part).double() - y).abs() <= bound(x[:, :96].double(), part.values().double(), y,
+                                                                            torch.bfloat16)).all()
 
 
 @pytest.mark.parametrize("T,N,K", [(1, 64, 96), (40, 257, 320), (300, 1024, 512), (513, 130, 1152), (257, 1, 64), (131, 903, 256)])
@@ -131,10 +147,11 @@ def test_gradient(T, N, K):
     assert (lhs - rhs).abs() <= slack
 
 
-def test_graphs_and_streams_side_by_side():
+@pytest.mark.parametrize("tokens", [(1, 16, 40), (300, 5, 2100), (128, 2500, 64)])
+def test_graphs_and_streams_side_by_side(tokens):
     """Two captured graphs and eager calls of the same weight at once: no shared scratch."""
     W = weight(1536, 2048, seed=3)
-    xs = [rand(t, 2048, seed=t).bfloat16() for t in (1, 16, 40)]
+    xs = [rand(t, 2048, seed=t).bfloat16() for t in tokens]
     want = [quant.linear_fp4(x, W) for x in xs]
     graphs = []
     for x in xs[:2]:
