@@ -11,6 +11,23 @@
 namespace gq4 {
 using namespace gk;
 
+// For kernels that wait before they touch memory: set up while the kernel in front drains, decode chain or not (a product with a
+// kernel in front of it that prepares its tokens starts 2 us sooner).
+template <typename... KArgs, typename... Args>
+inline int launch_waiting(void (*kernel)(KArgs...), unsigned grid, cudaStream_t st, Args... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid, 1, 1);
+  cfg.blockDim = dim3(256, 1, 1);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
+  return gk::launch_status();
+}
+
 inline unsigned grid_for(long long units) {
   const long long want = (units + 255) / 256, most = gk::sm_count() * 32ll;
   return static_cast<unsigned>(want < most ? want : most);
@@ -120,6 +137,7 @@ struct Fp4Params {
   int out_fp32;
   const void* bias;
   int bias_fp32;
+  int early;                                   // the weight may be read before the kernel in front has ended
   int* err;
 };
 
@@ -285,7 +303,7 @@ fp4_decode_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant
     fence_barrier_init();
     if (p.ks > 1) mbar_expect_tx(rfull, (p.ks - 1) * cs * BM * 4);
     pre = kblocks < p.stages ? kblocks : p.stages;
-    // the weight does not depend on the kernel in front
+    if (!p.early) pdl_wait();
     for (int kb = 0; kb < pre; ++kb) load_weight(kb, kb);
     pdl_wait();
     for (int kb = 0; kb < pre; ++kb) load_tokens(kb, kb);
@@ -975,7 +993,10 @@ inline int decode_launch(const void* codes, const void* xq, long long xq_rows, i
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
   attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[1].val.programmaticStreamSerializationAllowed = pl.src == SPLIT || gk::pdl_flag();   // behind the split of the same call
+  // Set up while the kernel in front drains.  What that kernel may have written is read behind the wait; the weight only where it
+  // cannot have: behind the split of the same call, in a decode chain.
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  p.early = pl.src == SPLIT || gk::pdl_flag();
   cfg.attrs = attr;
   cfg.numAttrs = 2;
   if (cudaLaunchKernelEx(&cfg, kernel, tmW, tmX, p) != cudaSuccess)
@@ -1056,8 +1077,8 @@ GK_EXPORT int gk_fp4_product(const void* codes, const void* tiles, const void* x
     uint8_t* sf = ws + rows * Kp;
     p.sf = sf;
     const SplitLayout lay = {T, pl.Tc, pl.Tp, K, Kp, kb * pl.nsf, pl.nsf, 1};
-    gk::launch_k(fp4_split_kernel, dim3(split_grid), dim3(256), 0, st, static_cast<const uint4*>(x), reinterpret_cast<uint2*>(ws), sf, lay);
-    if (int rc = gk::launch_status()) return rc;
+    if (int rc = launch_waiting(fp4_split_kernel, split_grid, st, static_cast<const uint4*>(x), reinterpret_cast<uint2*>(ws), sf, lay))
+      return rc;
     return decode_launch(codes, ws, rows, Kp, pl, p, st);
   }
   if (!ws) return -2;
@@ -1069,9 +1090,9 @@ GK_EXPORT int gk_fp4_product(const void* codes, const void* tiles, const void* x
   p.Y = Y; p.ldy = ldy; p.out_fp32 = out_fp32; p.bias = bias; p.bias_fp32 = bias_fp32; p.err = err;
   if (terms == 1) {
     p.sf = ws;
-    gk::launch_k(fp4_tiles_kernel, dim3(grid_for(static_cast<long long>(T) * kb)), dim3(256), 0, st, static_cast<const uint8_t*>(xs),
-                 ws, T, K / 32, kb);
-    if (int rc = gk::launch_status()) return rc;
+    if (int rc = launch_waiting(fp4_tiles_kernel, grid_for(static_cast<long long>(T) * kb), st, static_cast<const uint8_t*>(xs), ws, T,
+                                K / 32, kb))
+      return rc;
     return prompt_launch<1>(codes, x, T, K, p, Kp, st);
   }
   const int rows = mt * PM;
@@ -1079,7 +1100,7 @@ GK_EXPORT int gk_fp4_product(const void* codes, const void* tiles, const void* x
   p.sf = sf;
   p.lo_rows = rows;
   const SplitLayout lay = {T, rows, rows, K, Kp, 0, 1, kb};
-  gk::launch_k(fp4_split_kernel, dim3(split_grid), dim3(256), 0, st, static_cast<const uint4*>(x), reinterpret_cast<uint2*>(ws), sf, lay);
-  if (int rc = gk::launch_status()) return rc;
+  if (int rc = launch_waiting(fp4_split_kernel, split_grid, st, static_cast<const uint4*>(x), reinterpret_cast<uint2*>(ws), sf, lay))
+    return rc;
   return prompt_launch<2>(codes, ws, 2ll * rows, Kp, p, Kp, st);
 }
