@@ -11,23 +11,6 @@
 namespace gq4 {
 using namespace gk;
 
-// For kernels that wait before they touch memory: set up while the kernel in front drains, decode chain or not (a product with a
-// kernel in front of it that prepares its tokens starts 2 us sooner).
-template <typename... KArgs, typename... Args>
-inline int launch_waiting(void (*kernel)(KArgs...), unsigned grid, cudaStream_t st, Args... args) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(grid, 1, 1);
-  cfg.blockDim = dim3(256, 1, 1);
-  cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
-  return gk::launch_status();
-}
-
 inline unsigned grid_for(long long units) {
   const long long want = (units + 255) / 256, most = gk::sm_count() * 32ll;
   return static_cast<unsigned>(want < most ? want : most);
@@ -725,7 +708,8 @@ fp4_prompt_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant
 #pragma unroll
         for (int c = 0; c < 128; ++c) {
           const int col = col0 + c < p.N ? col0 + c : p.N - 1;
-          const float b = p.bias_fp32 ? static_cast<const float*>(p.bias)[col] : __bfloat162float(static_cast<const __nv_bfloat16*>(p.bias)[col]);
+          const float b = p.bias_fp32 ? static_cast<const float*>(p.bias)[col]
+                                      : __bfloat162float(static_cast<const __nv_bfloat16*>(p.bias)[col]);
           r[c >> 5][c & 31] = __float_as_uint(__uint_as_float(r[c >> 5][c & 31]) + b);
         }
       }
@@ -834,7 +818,8 @@ fp4_prompt_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant
 // codes [N, K / 2], tiles [ceil(N / 128), K / 128, 512], out [rows, K] bf16, zero from row N on; N <= rows, both in the same last
 // tile; K a multiple of 128, 16-byte aligned.
 GK_EXPORT int gk_fp4_dequant(const void* codes, const void* tiles, void* out, long long N, long long rows, int K, void* stream) {
-  if (N < 0 || rows < N || (rows + 127) / 128 != (N + 127) / 128 || K <= 0 || K % 128 || ((reinterpret_cast<uintptr_t>(codes) | reinterpret_cast<uintptr_t>(out)) & 15)) return -1;
+  if (N < 0 || rows < N || (rows + 127) / 128 != (N + 127) / 128 || K <= 0 || K % 128) return -1;
+  if (((reinterpret_cast<uintptr_t>(codes) | reinterpret_cast<uintptr_t>(out)) & 15)) return -1;
   const long long ctas = (N + 127) / 128 * (K / 128);
   if (ctas == 0) return 0;
   if (ctas > 0x7fffffffll) return -3;
@@ -900,11 +885,11 @@ struct Fp4Plan {
 // The decode kernel's plan: tokens per CTA (`Tc`, in whole columns of the product), how many CTAs share a tile's K, how deep the
 // ring is.  The cheapest by a model of what was measured (B200, us).  A K block of a lone CTA takes 0.26 (the issuing warp's
 // chain) or 0.0085 a KB of operands (60 bytes a cycle, what an SM gets out of L2); two CTAs on an SM share its 0.2 of the memory's
-// rate; all together get 9.5 KB a ns out of L2.  A round of CTAs costs 2 and Tc / 50 for each CTA of an SM, a launch 2, the exchange in a cluster 2 +
-// Tc / 33 and 1 more for eight CTAs, of which fewer fit into a GPC.  Chosen against the others that were run, ks = 1 / 2 / 4 / 8: 1 x
-// 4608 x 3584 12.0 / 9.5 / [9.0] / 9.8, 64 x 4608 x 3584 [14.1] / 14.6 / 21.0 / 26.1, 64 x 3584 x 18944 45.7 / 31.8 / [20.6] / 27.6, 16 x
-// 3584 x 18944 - / 25.4 / 16.7 / [15.2], 96 x 28672 x 4096 (e4m3) [23.1] / 67 / 89 / 154; one or two CTAs an SM: 1 x 37888 x 3584 22.6 /
-// [16.0], 64 x 4608 x 3584 [14.1] / 16.3.
+// rate; all together get 9.5 KB a ns out of L2.  A round of CTAs costs 2 and Tc / 50 for each CTA of an SM, a launch 2, the
+// exchange in a cluster 2 + Tc / 33 and 1 more for eight CTAs, of which fewer fit into a GPC.  Chosen against the others that were
+// run, ks = 1 / 2 / 4 / 8: 1 x 4608 x 3584 12.0 / 9.5 / [9.0] / 9.8, 64 x 4608 x 3584 [14.1] / 14.6 / 21.0 / 26.1, 64 x 3584 x 18944
+// 45.7 / 31.8 / [20.6] / 27.6, 16 x 3584 x 18944 - / 25.4 / [16.7] / 15.2, 96 x 28672 x 4096 (e4m3) [23.1] / 67 / 89 / 154; one or two
+// CTAs an SM: 1 x 37888 x 3584 22.6 / [16.0], 64 x 4608 x 3584 [14.1] / 16.3.
 inline Fp4Plan decode_plan(int T, int Tc, int terms, int N, int kb) {
   Fp4Plan p = {}, best = {};
   p.T = T;
@@ -1077,7 +1062,8 @@ GK_EXPORT int gk_fp4_product(const void* codes, const void* tiles, const void* x
     uint8_t* sf = ws + rows * Kp;
     p.sf = sf;
     const SplitLayout lay = {T, pl.Tc, pl.Tp, K, Kp, kb * pl.nsf, pl.nsf, 1};
-    if (int rc = launch_waiting(fp4_split_kernel, split_grid, st, static_cast<const uint4*>(x), reinterpret_cast<uint2*>(ws), sf, lay))
+    if (int rc = gk::launch_waiting(fp4_split_kernel, split_grid, 256, st, static_cast<const uint4*>(x),
+                                    reinterpret_cast<uint2*>(ws), sf, lay))
       return rc;
     return decode_launch(codes, ws, rows, Kp, pl, p, st);
   }
@@ -1090,8 +1076,8 @@ GK_EXPORT int gk_fp4_product(const void* codes, const void* tiles, const void* x
   p.Y = Y; p.ldy = ldy; p.out_fp32 = out_fp32; p.bias = bias; p.bias_fp32 = bias_fp32; p.err = err;
   if (terms == 1) {
     p.sf = ws;
-    if (int rc = launch_waiting(fp4_tiles_kernel, grid_for(static_cast<long long>(T) * kb), st, static_cast<const uint8_t*>(xs), ws, T,
-                                K / 32, kb))
+    if (int rc = gk::launch_waiting(fp4_tiles_kernel, grid_for(static_cast<long long>(T) * kb), 256, st,
+                                    static_cast<const uint8_t*>(xs), ws, T, K / 32, kb))
       return rc;
     return prompt_launch<1>(codes, x, T, K, p, Kp, st);
   }
@@ -1100,7 +1086,8 @@ GK_EXPORT int gk_fp4_product(const void* codes, const void* tiles, const void* x
   p.sf = sf;
   p.lo_rows = rows;
   const SplitLayout lay = {T, rows, rows, K, Kp, 0, 1, kb};
-  if (int rc = launch_waiting(fp4_split_kernel, split_grid, st, static_cast<const uint4*>(x), reinterpret_cast<uint2*>(ws), sf, lay))
+  if (int rc = gk::launch_waiting(fp4_split_kernel, split_grid, 256, st, static_cast<const uint4*>(x), reinterpret_cast<uint2*>(ws),
+                                  sf, lay))
     return rc;
   return prompt_launch<2>(codes, ws, 2ll * rows, Kp, p, Kp, st);
 }

@@ -169,6 +169,24 @@ inline void launch_k(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t sme
   cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
 }
 
+inline int launch_status();
+// The same outside a decode chain too, for kernels that wait before they touch anything that the kernel in front may have written:
+// their set-up overlaps its tail (a product behind the kernel that prepares its tokens starts 2 us sooner).
+template <typename... KArgs, typename... Args>
+inline int launch_waiting(void (*kernel)(KArgs...), unsigned grid, unsigned block, cudaStream_t st, Args... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid, 1, 1);
+  cfg.blockDim = dim3(block, 1, 1);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
+  return launch_status();
+}
+
 inline int launch_status() {
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) {

@@ -233,22 +233,6 @@ __global__ void __launch_bounds__(256) rows_quant_kernel(const Row8* __restrict_
   }
 }
 
-// Set up while the kernel in front drains, decode chain or not: the kernels wait before they read what it may have written.
-template <typename... KArgs, typename... Args>
-inline int launch_waiting(void (*kernel)(KArgs...), unsigned grid, void* stream, Args... args) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(grid, 1, 1);
-  cfg.blockDim = dim3(256, 1, 1);
-  cfg.stream = static_cast<cudaStream_t>(stream);
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
-  return gk::launch_status();
-}
-
 inline bool aligned16(const void* a) { return (reinterpret_cast<uintptr_t>(a) & 15) == 0; }
 
 }  // namespace gqr
@@ -264,9 +248,9 @@ GK_EXPORT int gk_norm_quant(const void* x, const void* res, const void* w, void*
   if (T == 0) return 0;
   const int sms = gk::sm_count(), grid = T < sms * 8 ? T : sms * 8, nv = H / 8;
   auto go = [&](auto kernel) {
-    return launch_waiting(kernel, grid, stream, static_cast<const Row8*>(x), static_cast<const Row8*>(res),
-                          static_cast<const Row8*>(w), static_cast<uint2*>(q), scales, static_cast<Row8*>(res_out), T, H, eps,
-                          gk::pdl_flag());
+    return gk::launch_waiting(kernel, grid, 256, static_cast<cudaStream_t>(stream), static_cast<const Row8*>(x),
+                              static_cast<const Row8*>(res), static_cast<const Row8*>(w), static_cast<uint2*>(q), scales,
+                              static_cast<Row8*>(res_out), T, H, eps, gk::pdl_flag());
   };
   auto slots = [&](auto sc, auto as) {
     constexpr bool S = decltype(sc)::value, A = decltype(as)::value;
@@ -293,8 +277,8 @@ GK_EXPORT int gk_rows_quant(const void* in, void* q, void* scales, long long T, 
   const bool two = units > gk::sm_count() * 2048ll;
   const long long blocks = two ? (units + 511) / 512 : (units + 255) / 256;
   auto go = [&](auto kernel, auto n) {
-    return launch_waiting(kernel, static_cast<unsigned>(blocks < most ? blocks : most), stream, static_cast<const Row8*>(in),
-                          static_cast<uint2*>(q), scales, n, nv);
+    return gk::launch_waiting(kernel, static_cast<unsigned>(blocks < most ? blocks : most), 256, static_cast<cudaStream_t>(stream),
+                              static_cast<const Row8*>(in), static_cast<uint2*>(q), scales, n, nv);
   };
   auto pick = [&](auto width, auto n) {
     using I = decltype(n);
