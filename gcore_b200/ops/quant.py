@@ -473,7 +473,7 @@ def gemm_fp4(a_q: torch.Tensor, a_s: torch.Tensor, weight: Fp4Weight, bias: torc
     N, K = weight.shape
     if tuple(a_s.shape) != (*a_q.shape[:-1], K // 32) or a_s.device != a_q.device:
         raise ValueError(f"gemm_fp4: scales {tuple(a_s.shape)} on {a_s.device} for activations {tuple(a_q.shape)} on {a_q.device}")
-    if bias is not None and bias.requires_grad and torch.is_grad_enabled():
+    if torch.is_grad_enabled() and (a_q.requires_grad or a_s.requires_grad or (bias is not None and bias.requires_grad)):
         raise RuntimeError("gemm_fp4 has no gradient: call it under torch.no_grad()")
     if out_dtype not in (torch.bfloat16, torch.float32):
         raise ValueError(f"gemm_fp4: results are bfloat16 or float32, not {out_dtype}")

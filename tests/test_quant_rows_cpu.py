@@ -137,3 +137,14 @@ def test_single_rows_without_a_batch():
     W = quant.Fp4Weight.of(rows(8, 256, 1))
     q, s = quant.quant_act_1x32(x)
     assert quant.linear_fp4(x, W).shape == (8,) and quant.gemm_fp4(q, s, W).shape == (8,)
+
+
+def test_gemm_fp4_refuses_activations_and_scales_that_want_a_gradient():
+    q, s = quant.quant_act_1x32(rows(3, 64, 5))
+    W = quant.Fp4Weight.of(rows(8, 64, 6))
+    with pytest.raises(RuntimeError, match="no gradient"):
+        quant.gemm_fp4(q.clone().requires_grad_(), s, W)
+    with pytest.raises(RuntimeError, match="no gradient"):
+        quant.gemm_fp4(q, s.clone().requires_grad_(), W)
+    with torch.no_grad():
+        assert torch.equal(quant.gemm_fp4(q.clone().requires_grad_(), s, W), quant.gemm_fp4(q, s, W))
