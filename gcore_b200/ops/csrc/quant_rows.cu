@@ -272,7 +272,8 @@ GK_EXPORT int gk_rows_quant(const void* in, void* q, void* scales, long long T, 
   if (!aligned16(in) || !aligned16(q)) return -2;
   if (T == 0) return 0;
   const int nv = F / 8;
-  // two units under way per thread once every thread of the GPU has one (us, one / two: 8191 x 14336 101.7 / 99.5, 64 x 18944 3.6 / 3.9)
+  // two units under way per thread once every thread of the GPU has one (us, one / two, before the units' rows shared a division:
+  // 8191 x 14336 101.7 / 99.5, 64 x 18944 3.6 / 3.9; as it stands 91 and 3.0 in a graph)
   const long long units = T * nv, most = gk::sm_count() * 32ll;
   const bool two = units > gk::sm_count() * 2048ll;
   const long long blocks = two ? (units + 511) / 512 : (units + 255) / 256;
