@@ -984,9 +984,7 @@ inline int decode_launch(const void* codes, const void* xq, long long xq_rows, i
   p.early = pl.src == SPLIT || gk::pdl_flag();
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  if (cudaLaunchKernelEx(&cfg, kernel, tmW, tmX, p) != cudaSuccess)
-    return gk::launch_status() ? gk::launch_status() : -14;
-  return gk::launch_status();
+  return gk::launch_ex(cfg, kernel, tmW, tmX, p);
 }
 
 }  // namespace gq4
@@ -1012,9 +1010,7 @@ inline int prompt_launch(const void* codes, const void* xq, long long xq_rows, i
   attr[0].val.programmaticStreamSerializationAllowed = 1;   // behind the kernel of the same call that prepares the tokens
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  if (cudaLaunchKernelEx(&cfg, fp4_prompt_kernel<TERMS>, tmW, tmX, p) != cudaSuccess)
-    return gk::launch_status() ? gk::launch_status() : -14;
-  return gk::launch_status();
+  return gk::launch_ex(cfg, fp4_prompt_kernel<TERMS>, tmW, tmX, p);
 }
 }  // namespace gq4
 

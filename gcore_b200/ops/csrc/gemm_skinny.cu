@@ -309,6 +309,5 @@ GK_EXPORT int gk_gemm_skinny(const void* W, long long ldw, const void* X, long l
   attr[1].val.programmaticStreamSerializationAllowed = gk::pdl_flag() ? 1 : 0;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  if (cudaLaunchKernelEx(&cfg, gemm_skinny_kernel, tmW, tmX, p) != cudaSuccess) return gk::launch_status() ? gk::launch_status() : -7;
-  return gk::launch_status();
+  return gk::launch_ex(cfg, gemm_skinny_kernel, tmW, tmX, p);
 }

@@ -169,7 +169,23 @@ inline void launch_k(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t sme
   cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
 }
 
-inline int launch_status();
+inline int launch_status() {
+  cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) {
+    fprintf(stderr, "[gcore_b200] kernel launch failed: %s\n", cudaGetErrorString(e));
+    return static_cast<int>(e);
+  }
+  return 0;
+}
+
+// A launch and its status: not zero where the launch failed.  Asking takes most errors off the runtime, so it is asked once.
+template <typename... KArgs, typename... Args>
+inline int launch_ex(const cudaLaunchConfig_t& cfg, void (*kernel)(KArgs...), Args... args) {
+  const cudaError_t rc = cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
+  const int status = launch_status();
+  return rc == cudaSuccess || status ? status : static_cast<int>(rc);
+}
+
 // The same outside a decode chain too, for kernels that wait before they touch anything that the kernel in front may have written:
 // their set-up overlaps its tail (a product behind the kernel that prepares its tokens starts 2 us sooner).
 template <typename... KArgs, typename... Args>
@@ -183,17 +199,7 @@ inline int launch_waiting(void (*kernel)(KArgs...), unsigned grid, unsigned bloc
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
-  return launch_status();
-}
-
-inline int launch_status() {
-  cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess) {
-    fprintf(stderr, "[gcore_b200] kernel launch failed: %s\n", cudaGetErrorString(e));
-    return static_cast<int>(e);
-  }
-  return 0;
+  return launch_ex(cfg, kernel, args...);
 }
 
 }  // namespace gk
