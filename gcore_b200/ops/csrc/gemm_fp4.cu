@@ -16,6 +16,12 @@ inline unsigned grid_for(long long units) {
   return static_cast<unsigned>(want < most ? want : most);
 }
 
+// A product whose operands and result may be below 2^-126 (the file is compiled with such values flushed to zero).
+__device__ __forceinline__ float times(float a, float b) {
+  float c;
+  asm("mul.rn.f32 %0, %1, %2;" : "=f"(c) : "f"(a), "f"(b));
+  return c;
+}
 // 2^(e - 127); 255 is NaN.  2^-127 and values below 2^-126 become zero (subnormals are flushed).
 __device__ __forceinline__ float pow2_of(uint32_t e) {
   return e == 255u ? __uint_as_float(0x7fffffffu) : __uint_as_float(e << 23);
@@ -214,7 +220,7 @@ __device__ __forceinline__ Terms split8(const uint4& raw) {
   uint32_t hi[4], lo[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const float a = __uint_as_float(w[i] << 16) * inv, b = __uint_as_float(w[i] & 0xffff0000u) * inv;
+    const float a = times(__uint_as_float(w[i] << 16), inv), b = times(__uint_as_float(w[i] & 0xffff0000u), inv);
     hi[i] = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
     const __half2 h = __half2(__nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(hi[i]), __NV_E4M3));
     lo[i] = __nv_cvt_float2_to_fp8x2(make_float2((a - __low2float(h)) * 16.f, (b - __high2float(h)) * 16.f), __NV_SATFINITE,
