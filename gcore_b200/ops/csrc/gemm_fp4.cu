@@ -93,8 +93,9 @@ __global__ void __launch_bounds__(256) pad_rows16_kernel(const uint32_t* __restr
 //     cycles for 16 columns as for 128, and its operands' and descriptors' way to the tensor core is what the issuing warp spends
 //     its time on: with one lane in a branch of its own 64 tokens of 3584 x 18944 took 79 us in one piece, now 46.
 //   * 16-bit activations enter as two e4m3 terms, x = 2^e (hi + lo / 16) with one e per 32 values: hi keeps four significant bits, lo
-//     the four behind them, so a bf16 value at most 2^14 below its group's largest is exact and a smaller one is off by less
-//     than 2^-22 of that largest.  The terms are separate columns of one product; the epilogue adds them.
+//     the four behind them down to a step of 2^-9, 2^-13 of hi's unit.  With the group's largest between 224 and 448 of it a
+//     bf16 value at most 2^13 below that largest is exact, and a smaller one is off by less than 2^-21 of it (half a step, 2^-14,
+//     of 224).  The terms are separate columns of one product; the epilogue adds them.
 //   * K is divided over a cluster of `ks` CTAs where there are few tiles: CTA r finishes tokens r, r + ks, ..., whose partial sums
 //     the others send it through distributed shared memory in one copy each (stores of 128 bytes a warp took 20 us for 64
 //     tokens); it adds them in the order of the CTAs.
@@ -212,9 +213,8 @@ __device__ __forceinline__ Terms split8(const uint4& raw) {
   top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
   top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
   // bf16 pattern of the largest: eight bits of exponent, seven of mantissa; 448 = 1.75 * 2^8 as in quant_rows.cu.  The lo term's
-  // exponent is four less, so the hi term's is at least 4 (values below 2^-114 lose bits there).
-  uint32_t e = (top >> 7) - 8u + ((top & 0x7fu) > 0x60u ? 1u : 0u);
-  if (top < (13u << 7)) e = 4u;
+  // exponent is four less, so the hi term's is at least 4: a group whose largest is below 2^-115 keeps steps of 2^-136.
+  const uint32_t e = static_cast<uint32_t>(max(static_cast<int>(top >> 7) - 8 + ((top & 0x7fu) > 0x60u ? 1 : 0), 4));
   const bool bad = top >= 0x7f80u;
   const float inv = __uint_as_float((254u - (bad ? 127u : e)) << 23);
   uint32_t hi[4], lo[4];

@@ -19,7 +19,7 @@ def large_weight(N, K, exponent):
 
 
 @pytest.mark.parametrize("T", [1, 5, 40, 200])
-@pytest.mark.parametrize("exponent", [1, 4, 10, 11])
+@pytest.mark.parametrize("exponent", [1, 4, 10, 11, 12, 13, 14])
 def test_groups_of_tiny_values(T, exponent):
     """The largest of each group has this biased exponent and a mantissa on either side of e4m3's largest, 1.75."""
     N, K = 130, 256
