@@ -22,16 +22,16 @@ __device__ __forceinline__ float times(float a, float b) {
   asm("mul.rn.f32 %0, %1, %2;" : "=f"(c) : "f"(a), "f"(b));
   return c;
 }
-// 2^(e - 127); 255 is NaN.  2^-127 and values below 2^-126 become zero (subnormals are flushed).
+// 2^(e - 127); 255 is NaN.
 __device__ __forceinline__ float pow2_of(uint32_t e) {
-  return e == 255u ? __uint_as_float(0x7fffffffu) : __uint_as_float(e << 23);
+  return __uint_as_float(e == 255u ? 0x7fffffffu : e == 0u ? 0x400000u : e << 23);
 }
 __device__ __forceinline__ uint32_t two_bf16(float a, float b) {
   const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
   return *reinterpret_cast<const uint32_t*>(&v);
 }
 
-// bf16 values (exact: two significant bits) of the weight.  A CTA per tile of 128 x 128: sixteen threads a row, eight values each,
+// bf16 values of the weight (exact: two significant bits; infinity from 2^128 on).  A CTA per tile of 128 x 128: sixteen threads a row, eight values each,
 // eight rows a thread, so that a warp writes whole lines and eight loads are under way.  Two and a half bytes a value: 6144 x
 // 4096 12.3 us (floor 9.9; one row a thread and a division each 22.7).
 __global__ void __launch_bounds__(256) fp4_dequant_kernel(const uint32_t* __restrict__ codes, const uint8_t* __restrict__ tiles,
@@ -53,7 +53,7 @@ __global__ void __launch_bounds__(256) fp4_dequant_kernel(const uint32_t* __rest
 #pragma unroll
     for (int b = 0; b < 4; ++b) {
       const __half2 h = __half2(__nv_cvt_fp4x2_to_halfraw2(static_cast<__nv_fp4x2_storage_t>(w[i] >> (8 * b)), __NV_E2M1));
-      o[b] = two_bf16(__low2float(h) * s, __high2float(h) * s);
+      o[b] = two_bf16(times(__low2float(h), s), times(__high2float(h), s));
     }
     out[at + i * step] = make_uint4(o[0], o[1], o[2], o[3]);
   }

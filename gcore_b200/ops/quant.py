@@ -361,7 +361,7 @@ class Fp4Weight:
         return out
 
     def values(self, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
-        """The weight [N, K] in ``dtype`` (bf16 holds every value; the result may be a view of wider rows)."""
+        """The weight [N, K] in ``dtype`` (bf16 holds every value below 2^128; the result may be a view of wider rows)."""
         N, K = self.shape
         if dtype == torch.bfloat16 and _lib.use_native(self.codes):
             if not _lib.is_current(self.codes):
@@ -410,8 +410,8 @@ def _fp4_product(x2, xs, weight: Fp4Weight, bias, out_dtype):
 
 
 def _fp4_dgrad(dy, weight: Fp4Weight):
-    """``dy`` [T, N] times the weight [N, K]: its bf16 values, which are exact, on the framework's GEMM.  The product reads rows of
-    ``dy`` in 16-byte units: other widths get columns of zero, and the weight as many rows of zero."""
+    """``dy`` [T, N] times the weight [N, K]: its bf16 values, exact below 2^128, on the framework's GEMM.  The product reads rows
+    of ``dy`` in 16-byte units: other widths get columns of zero, and the weight as many rows of zero."""
     from .gemm import linear_dgrad
     (N, K), T = weight.shape, dy.shape[0]
     wide = (N + 7) // 8 * 8
