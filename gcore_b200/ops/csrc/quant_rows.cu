@@ -50,10 +50,24 @@ __device__ __forceinline__ float largest(float a, float b, float c) {
   return d;
 }
 
-// Eight values of a thread to codes; the 16 (SC32: 4) neighbouring lanes of its group hold the group's other values.  All lanes
-// of the warp call this; `unit` counts units of eight values over the whole matrix and picks the group's scale.
-template <bool SC32, bool AS16>
-__device__ __forceinline__ void quantise(float (&f)[8], bool live, long long unit, uint2* q, void* scales) {
+// The upper 22 of 24 bits, to nearest (Veltkamp's splitting).
+__device__ __forceinline__ float upper22(float t) {
+  const float c = __fmul_rn(t, 5.f);
+  return __fadd_rn(c, __fsub_rn(t, c));
+}
+
+// Eight values of a thread, f * unit, to codes; the 16 (SC32: 4) neighbouring lanes of its group hold the group's other values.
+// All lanes of the warp call this; `at` counts units of eight values over the whole matrix and picks the group's scale.
+//
+// fp32 scales of a norm that is not rounded in between (TIES): the code is that of f times 448 / amax, one division a group that
+// rounds to nearest.  f = x * gain * 2^n is the exact product of two bf16 values, and `unit`, what is left of the norm's factor, is
+// not in f / amax.  448 f / amax is then a ratio of 19 bits to 16, so either a tie between two codes (one value in 2 10^4 of bf16
+// rows) or more than 2^-21 away from one, 4.1 units in the last place; the product is off by 1.5 of them at most, and rounded to a
+// multiple of four it is a tie where the ratio is one, which goes to the even code.  3001 x 1536 values: 289 codes wrong where the
+// norm in 32 bits is multiplied by 1 / s, 269 where it is divided by s, none here; us, multiplied / here / a division for each
+// value: 3001 x 1536 6.9 / 7.9 / 14.0, 16384 x 4096 with residual 81.3 / 84.4 / 110.
+template <bool SC32, bool AS16, bool TIES>
+__device__ __forceinline__ void quantise(float (&f)[8], float unit, bool live, long long at, uint2* q, void* scales) {
   if (AS16) unpack(pack(f), f);
   if (SC32) {
     float amax = 1e-10f;
@@ -66,8 +80,8 @@ __device__ __forceinline__ void quantise(float (&f)[8], bool live, long long uni
     const uint32_t e = top >= 0x7f800000u ? 255u : (top >> 23) - 8u + ((top & 0x7fffffu) > 0x600000u ? 1u : 0u);
     const float inv = __uint_as_float((254u - min(e, 253u)) << 23);
     if (live) {
-      q[unit] = codes8(f, inv);
-      if ((threadIdx.x & 3) == 0) static_cast<uint8_t*>(scales)[unit >> 2] = static_cast<uint8_t>(e);
+      q[at] = codes8(f, inv);
+      if ((threadIdx.x & 3) == 0) static_cast<uint8_t*>(scales)[at >> 2] = static_cast<uint8_t>(e);
     }
   } else {
     float amax = fabsf(f[0]);
@@ -75,11 +89,23 @@ __device__ __forceinline__ void quantise(float (&f)[8], bool live, long long uni
     for (int j = 1; j < 8; ++j) amax = fmaxf(amax, fabsf(f[j]));
 #pragma unroll
     for (int o = 8; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-    const float s = fmaxf(amax, 1e-10f) / 448.f;
-    const float inv = 1.f / s;
+    float s, inv = 1.f;
+    if (AS16 || !TIES) {   // as the chain's quantiser computes them: 2^-22, less than an activation is off
+      s = fmaxf(amax, 1e-10f) / 448.f;
+      inv = 1.f / s;
+    } else {
+      // one division for both: the scale in the lane that stores it, 448 / amax in the others
+      const bool lead = (threadIdx.x & 15) == 0;
+      const float top = amax * unit, under = top > 1e-10f ? amax : 1e-10f / unit;
+      s = __fdiv_rn(lead ? fmaxf(top, 1e-10f) : 448.f, lead ? 448.f : under);
+      inv = __shfl_sync(0xffffffffu, s, (threadIdx.x & 16) | 1);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) f[j] = upper22(__fmul_rn(f[j], inv));
+      inv = 1.f;
+    }
     if (live) {
-      q[unit] = codes8(f, inv);
-      if ((threadIdx.x & 15) == 0) static_cast<float*>(scales)[unit >> 4] = s;
+      q[at] = codes8(f, inv);
+      if ((threadIdx.x & 15) == 0) static_cast<float*>(scales)[at >> 4] = s;
     }
   }
 }
@@ -103,7 +129,7 @@ template <int SLOTS, bool SC32, bool AS16>
 __global__ void __launch_bounds__(256) norm_quant_kernel(const Row8* __restrict__ x, const Row8* __restrict__ res,
                                                          const Row8* __restrict__ w, uint2* __restrict__ q,
                                                          void* __restrict__ scales, Row8* __restrict__ res_out, int T, int H,
-                                                         float eps, int early) {
+                                                         float eps, float inv_h, int early) {
   __shared__ float red[32];
   pdl_launch_dependents();
   if (!early) pdl_wait();   // the gains may be read before the kernel in front has ended in a decode chain only
@@ -160,7 +186,12 @@ __global__ void __launch_bounds__(256) norm_quant_kernel(const Row8* __restrict_
       }
     }
     ss = block_sum(ss, red);
-    const float rstd = rsqrtf(ss / H + eps);
+    float factor = rsqrtf((AS16 ? ss / H : ss * inv_h) + eps), unit = 1.f;
+    if (!SC32 && !AS16) {   // the power of two and, in `unit`, the rest; zero, infinity and NaN as they are
+      const uint32_t bits = __float_as_uint(factor);
+      unit = __uint_as_float((bits & 0x7fffffu) | 0x3f800000u);
+      if (bits < 0x7f800000u) factor = __uint_as_float(bits & 0x7f800000u);
+    }
 #pragma unroll
     for (int s = 0; s < SLOTS; ++s) {
       const int i = threadIdx.x + s * 256;
@@ -170,9 +201,9 @@ __global__ void __launch_bounds__(256) norm_quant_kernel(const Row8* __restrict_
         unpack(v[s], f);
         if (!WIDE) unpack(gain[s], g);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) f[j] = f[j] * rstd * (WIDE ? gain32[WIDE ? s : 0][j] : g[j]);
+        for (int j = 0; j < 8; ++j) f[j] = f[j] * factor * (WIDE ? gain32[WIDE ? s : 0][j] : g[j]);
       }
-      quantise<SC32, AS16>(f, i < nv, at + i, q, scales);
+      quantise<SC32, AS16, true>(f, unit, i < nv, at + i, q, scales);
     }
   }
 }
@@ -228,7 +259,7 @@ __global__ void __launch_bounds__(256) rows_quant_kernel(const Row8* __restrict_
           }
         }
       }
-      quantise<SC32, AS16>(f, u < units, u, q, scales);
+      quantise<SC32, AS16, false>(f, 1.f, u < units, u, q, scales);
     }
   }
 }
@@ -250,7 +281,7 @@ GK_EXPORT int gk_norm_quant(const void* x, const void* res, const void* w, void*
   auto go = [&](auto kernel) {
     return gk::launch_waiting(kernel, grid, 256, static_cast<cudaStream_t>(stream), static_cast<const Row8*>(x),
                               static_cast<const Row8*>(res), static_cast<const Row8*>(w), static_cast<uint2*>(q), scales,
-                              static_cast<Row8*>(res_out), T, H, eps, gk::pdl_flag());
+                              static_cast<Row8*>(res_out), T, H, eps, 1.f / static_cast<float>(H), gk::pdl_flag());
   };
   auto slots = [&](auto sc, auto as) {
     constexpr bool S = decltype(sc)::value, A = decltype(as)::value;
