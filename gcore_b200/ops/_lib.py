@@ -12,6 +12,7 @@ import os
 from pathlib import Path
 
 import torch
+import torch.autograd.forward_ad as forward_ad
 
 _HERE = Path(__file__).resolve().parent
 _KERNELS = None
@@ -115,6 +116,14 @@ def is_current(t: torch.Tensor) -> bool:
 def packed16(t: torch.Tensor) -> torch.Tensor:
     """``t`` itself where it is contiguous and starts on a 16-byte boundary, else a copy that is and does."""
     return t if t.is_contiguous() and t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
+
+
+def differentiated(*tensors) -> bool:
+    """Whether a derivative of one of the tensors (or None) is asked for: a gradient, or in forward mode a tangent."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        return True
+    return forward_ad._current_level >= 0 and any(
+        t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
 def check(rc: int, what: str):

@@ -348,7 +348,7 @@ def _check_e4m3_rows(what, width, scales, x, others=()):
     for t in others:
         if t is not None and t.device != x.device:
             raise ValueError(f"{what}: tensors on {x.device} and {t.device}")
-    if torch.is_grad_enabled() and (x.requires_grad or any(t is not None and t.requires_grad for t in others)):
+    if _lib.differentiated(x, *others):
         raise RuntimeError(f"{what} has no gradient: call it under torch.no_grad()")
 
 

@@ -427,9 +427,17 @@ class _LinearFp4(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x2, weight, bias):
         ctx.weight, ctx.bias_dtype = weight, bias.dtype if bias is not None else None
+        ctx.rows = x2.shape[0]
         return _fp4_product(x2, None, weight, bias, x2.dtype)
 
     @staticmethod
+    def jvp(ctx, x_t, _, bias_t):
+        if x_t is None:
+            return bias_t.to(torch.bfloat16).expand(ctx.rows, -1).clone()
+        return _fp4_product(_lib.packed16(x_t), None, ctx.weight, bias_t, x_t.dtype)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
         dx = db = None
         if ctx.needs_input_grad[0]:
@@ -445,7 +453,7 @@ class _LinearFp4(torch.autograd.Function):
 
 def linear_fp4(x: torch.Tensor, weight: Fp4Weight, bias: torch.Tensor | None = None) -> torch.Tensor:
     """``y = x W^T (+ bias)`` for a frozen 4-bit weight and 16-bit activations, ``x`` [..., K] -> [..., N] in ``x``'s type: the
-    product that a model trained with ``fp4_qat`` computes.  Differentiable in ``x`` and ``bias``."""
+    product that a model trained with ``fp4_qat`` computes.  Differentiable once in ``x`` and ``bias``, in reverse and forward mode."""
     _check_fp4("linear_fp4", x, weight, bias)
     N, K = weight.shape
     if not (_lib.use_native(x) and x.dtype == torch.bfloat16):
@@ -455,7 +463,7 @@ def linear_fp4(x: torch.Tensor, weight: Fp4Weight, bias: torch.Tensor | None = N
         with torch.cuda.device(x.device):
             return linear_fp4(x, weight, bias)
     x2 = _lib.packed16(x if x.dim() == 2 else x.reshape(-1, K))
-    if torch.is_grad_enabled() and (x.requires_grad or (bias is not None and bias.requires_grad)):
+    if _lib.differentiated(x, bias):
         y = _LinearFp4.apply(x2, weight, bias)
     else:
         y = _fp4_product(x2, None, weight, bias, x.dtype)
@@ -473,7 +481,7 @@ def gemm_fp4(a_q: torch.Tensor, a_s: torch.Tensor, weight: Fp4Weight, bias: torc
     N, K = weight.shape
     if tuple(a_s.shape) != (*a_q.shape[:-1], K // 32) or a_s.device != a_q.device:
         raise ValueError(f"gemm_fp4: scales {tuple(a_s.shape)} on {a_s.device} for activations {tuple(a_q.shape)} on {a_q.device}")
-    if torch.is_grad_enabled() and (a_q.requires_grad or a_s.requires_grad or (bias is not None and bias.requires_grad)):
+    if _lib.differentiated(a_q, a_s, bias):
         raise RuntimeError("gemm_fp4 has no gradient: call it under torch.no_grad()")
     if out_dtype not in (torch.bfloat16, torch.float32):
         raise ValueError(f"gemm_fp4: results are bfloat16 or float32, not {out_dtype}")
