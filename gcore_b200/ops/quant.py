@@ -289,16 +289,18 @@ def quant_rows_ref(y: torch.Tensor, scales: str):
 
 def quant_act_1x32(x: torch.Tensor):
     """``x`` [..., K] (K a multiple of 32) -> ``(q float8_e4m3fn [..., K], s float8_e8m0fnu [..., K / 32])``, the activations of
-    ``gemm_fp4``.  No gradient."""
+    ``gemm_fp4``.  Inference only."""
     K = x.shape[-1]
     if K == 0 or K % 32:
         raise ValueError(f"quant_act_1x32: a width of {K} is not a multiple of 32")
+    if _lib.differentiated(x):
+        raise RuntimeError("quant_act_1x32 has no gradient: call it under torch.no_grad()")
     if not (_lib.use_native(x) and x.dtype == torch.bfloat16):
-        return quant_rows_ref(x.detach(), "e8m0")
+        return quant_rows_ref(x, "e8m0")
     if not _lib.is_current(x):
         with torch.cuda.device(x.device):
             return quant_act_1x32(x)
-    x2 = _lib.packed16(x.detach())
+    x2 = _lib.packed16(x)
     q = torch.empty_like(x2, dtype=torch.float8_e4m3fn)
     s = torch.empty((*x.shape[:-1], K // 32), dtype=torch.float8_e8m0fnu, device=x.device)
     LAUNCHES["quant"] += 1

@@ -44,3 +44,15 @@ def test_product_carries_tangents_and_refuses_a_second_derivative(monkeypatch):
     g, = torch.autograd.grad(quant._LinearFp4.apply(x, W, None).square().sum(), x, create_graph=True)
     with pytest.raises(RuntimeError, match="once_differentiable"):   # not x's gradient alone, without the product's part
         (g.sum() + x.sum()).backward()
+
+
+def test_quantiser_refuses_a_gradient_and_a_tangent():
+    x = rows(3, 64, 1)
+    want = quant.quant_act_1x32(x)
+    with pytest.raises(RuntimeError, match="no gradient"):
+        quant.quant_act_1x32(x.clone().requires_grad_())
+    with fw.dual_level(), pytest.raises(RuntimeError, match="no gradient"):
+        quant.quant_act_1x32(fw.make_dual(x, x))
+    with torch.no_grad():
+        q, s = quant.quant_act_1x32(x.clone().requires_grad_())
+    assert not q.requires_grad and torch.equal(q.float(), want[0].float()) and torch.equal(s.float(), want[1].float())
