@@ -255,8 +255,8 @@ class InferEngineConfig(MappingMixin):
     attention_backend: str = "native"
     return_routed_experts: bool = False
     fp8_weights: bool = False
-    fp4_weights: bool = False          # dense projections served in 4 bits (what a policy trained with fp4_qat computes)
-    fp4_activations: str = "bf16"      # "bf16" | "fp8": what the 4-bit products read
+    fp4_weights: bool = False          # dense projections served in 4 bits (with policy.fp4_qat those that it trains with)
+    fp4_activations: str = "bf16"      # "bf16" (as they are) | "fp8": what the 4-bit products read
     watchdog_timeout: int = 600
     model_override_args: Dict[str, Any] = field(default_factory=dict)
     override_infer_engine_config: Dict[str, Any] = field(default_factory=dict)

@@ -222,8 +222,9 @@ class TrainingEngine:
             return
         from ..models.gpt import ParallelLinear
         from ..models.moe import Experts
+        from ..ops.lowp_linear import quantised_width
         for name, mod in self.model.named_modules():
-            if isinstance(mod, ParallelLinear) and "decoder.layers" in name and mod.in_local % 128 == 0 \
+            if isinstance(mod, ParallelLinear) and "decoder.layers" in name and quantised_width(mod.in_local) \
                     and mod.out_local > 1:
                 mod.precision = kind
                 self.lowp_modules.append(name)

@@ -22,6 +22,11 @@ from . import quant
 from .gemm import linear, linear_dgrad, linear_wgrad
 
 
+def quantised_width(columns: int) -> bool:
+    """Whether a projection of this contraction length trains in the policy's low precision (and is served in it)."""
+    return columns % 128 == 0
+
+
 def fake_quant_weight(w: torch.Tensor, kind: str) -> torch.Tensor:
     """Quantise -> dequantise copy of ``w`` (no gradient)."""
     with torch.no_grad():

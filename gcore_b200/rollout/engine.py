@@ -343,6 +343,7 @@ class InferEngine:
         self.record_routed_experts = False
         self._peer_ar = None
         self.fp4_activations: Optional[str] = None   # "bf16" | "fp8" when the engine serves 4-bit weights
+        self.fp4_as_trained = False
         self.weight_scales: dict = {}  # name -> fp32 128x128 block scales when weights are held in e4m3
 
     @property
@@ -482,7 +483,7 @@ class InferEngine:
         if getattr(self, "fp8_enabled", False):
             self.quantize_weights_fp8()
         if self.fp4_activations is not None:
-            self.quantize_weights_fp4(self.fp4_activations)
+            self.quantize_weights_fp4(self.fp4_activations, self.fp4_as_trained)
         for ent in self._mla_abs.values():
             ent[1] = True
         if self.device.type == "cuda":
@@ -506,22 +507,25 @@ class InferEngine:
         self._graphs.clear()
 
     # ------------------------------------------------------------------ 4-bit serving
-    def quantize_weights_fp4(self, activations: str = "bf16"):
+    def quantize_weights_fp4(self, activations: str = "bf16", as_trained: bool = False):
         """(Re)builds 4-bit copies (e2m1, one power of two per 32 columns) of every dense projection whose contraction length is a
-        multiple of 32; called after each weight hand-over like ``quantize_weights_fp8``.  ``activations="bf16"``: the products of
-        a policy trained with ``fp4_qat``, value for value; ``"fp8"``: the inputs are e4m3 with one power of two per 32 values."""
+        multiple of 32; called after each weight hand-over like ``quantize_weights_fp8``.  ``activations="bf16"``: the inputs stay as
+        they are; ``"fp8"``: they are e4m3 with one power of two per 32 values.  ``as_trained``: the weights that a policy with
+        ``fp4_qat`` multiplies with, value for value: the projections that it quantises (the others are served as they are), from
+        their own type; otherwise from bf16."""
+        from ..ops.lowp_linear import quantised_width
         from ..ops.quant import Fp4Weight
         if activations not in ("bf16", "fp8"):
             raise ValueError(f"activations of 4-bit serving are 'bf16' or 'fp8', got {activations!r}")
         if self.plan is not None:
             raise NotImplementedError("layer-plan decoders are served in bfloat16 or float32")
-        self.fp8_enabled, self.fp4_activations = False, activations
+        self.fp8_enabled, self.fp4_activations, self.fp4_as_trained = False, activations, as_trained
         for lw in self.w.layers:
             lw.fp8, lw.fp4 = None, {}
             for name in ("qkv_w", "o_w", "fc1_w", "fc2_w"):
                 w = getattr(lw, name)
-                if w is not None and w.dim() == 2 and w.shape[1] % 32 == 0:
-                    lw.fp4[name] = Fp4Weight.of(w.to(torch.bfloat16))
+                if w is not None and w.dim() == 2 and (quantised_width(w.shape[1]) if as_trained else w.shape[1] % 32 == 0):
+                    lw.fp4[name] = Fp4Weight.of(w if as_trained else w.to(torch.bfloat16))
         self._graphs.clear()
 
     def _input_scales(self, h, lw: LayerWeights, name: str) -> Optional[str]:

@@ -338,7 +338,7 @@ class GrpoTrainer:
         if self.serve_fp8:
             self.engine.quantize_weights_fp8()
         if self.serve_fp4:
-            self.engine.quantize_weights_fp4(self.fp4_activations)
+            self.engine.quantize_weights_fp4(self.fp4_activations, as_trained=self.cfg.policy.fp4_qat)
 
     def offload_model(self):
         """Trainable weights to pinned host memory (early-swap mode of the reference's ``OffloadManager``,
