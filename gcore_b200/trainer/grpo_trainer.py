@@ -75,8 +75,13 @@ class GrpoTrainer:
     # ------------------------------------------------------------------ setup
     def setup(self):
         cfg = self.cfg
-        self.policy.setup_model_and_get_optimizer()
         ie = cfg.sampler.infer_engine_configs[0]
+        if ie.fp4_weights and cfg.policy.fp8:
+            raise ValueError("the rollout engine serves its projections in 4 bits (fp4_weights) or in block fp8, not in both")
+        if ie.fp4_weights and cfg.policy.lora.enabled:
+            # the engine's weight is base + delta: rounded to 4 bits, most of a small delta goes and the rest is several times too large
+            raise ValueError("fp4_weights: a policy with LoRA adapters is not served in 4 bits, its adapters would be lost in the rounding")
+        self.policy.setup_model_and_get_optimizer()
         self.policy.temperature = ie.temperature
         if cfg.require_critic_model():
             self.critic = get_training_engine(cfg.critic, cfg.critic.optimizer, cfg.training, cfg.ppo,
@@ -124,8 +129,6 @@ class GrpoTrainer:
         # compute the same quantised products
         self.serve_fp8 = bool(getattr(ie, "fp8_weights", False) or cfg.policy.fp8)
         self.serve_fp4, self.fp4_activations = ie.fp4_weights, ie.fp4_activations
-        if self.serve_fp4 and self.serve_fp8:
-            raise ValueError("the rollout engine serves its projections in 4 bits (fp4_weights) or in block fp8, not in both")
         self._quantize_served_weights()
         self.engine.owns_weights = not share
         if getattr(cfg.policy, "offload_ref_model", False):

@@ -62,3 +62,13 @@ def test_a_policy_without_quantisation_is_served_in_4_bits_wherever_groups_are_w
     tr = trainer(qat=False, acts="fp8")
     assert set(tr.engine.w.layers[0].fp4) == {"qkv_w", "o_w", "fc1_w", "fc2_w"}
     assert tr.step(PROMPTS)["policy/grad_norm"] > 0
+
+
+def test_adapters_and_block_fp8_are_refused_before_anything_is_built():
+    with pytest.raises(ValueError, match="not in both"):
+        trainer(qat=False, fp8=True)
+    cfg = make_cfg()
+    cfg.policy.lora.rank = 8
+    for qat in (False, True):
+        with pytest.raises(ValueError, match="LoRA"):
+            trainer(qat=qat, lora=cfg.policy.lora)
