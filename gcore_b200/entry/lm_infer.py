@@ -30,6 +30,8 @@ def serve_checkpoint(cfg, inf):
     """Generation from a serving-only checkpoint through the rollout engine."""
     from ..checkpoint.hf import load_serving_model
     from ..rollout.engine import InferEngine, RolloutWeights, SamplingParams
+    if cfg.sampler.infer_engine_configs[0].fp4_weights:
+        raise NotImplementedError("fp4_weights: layer-plan decoders are served in bfloat16 or float32")
     if not torch.cuda.is_available():
         raise RuntimeError("serving a checkpoint needs a GPU")
     device = torch.device("cuda", torch.cuda.current_device())

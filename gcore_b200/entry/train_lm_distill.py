@@ -23,6 +23,8 @@ def off_policy_loop(trainer: GrpoTrainer, prompt_batches, steps: int, log):
     teacher's training-layout weights)."""
     cfg = trainer.cfg
     ie = cfg.sampler.infer_engine_configs[0]
+    if ie.fp4_weights:
+        raise NotImplementedError("fp4_weights: the teacher of an off-policy distillation is served as it is")
     teacher = trainer.teacher
     eng = InferEngine(teacher.model_cfg, RolloutWeights.from_model(teacher.model), tp_size=teacher.model.tp_size,
                       max_running_requests=ie.max_running_requests or cfg.training.rollout_gbs,

@@ -202,11 +202,18 @@ def recv_weights(infer_engine: InferEngine, model_for_names, layout: RoleLayout)
 
 
 # ---------------------------------------------------------------------------------------------------- rollout ranks
+def check_serving(ie):
+    """Both sides of the job ask this before they wait for one another."""
+    if ie.fp4_weights:
+        raise NotImplementedError("fp4_weights: remote rollout engines serve the weights as they are sent")
+
+
 class SamplerServer:
     """What a rollout rank runs: an engine with weights of its own, served until the trainers say stop."""
 
     def __init__(self, cfg, model_cfg, layout: RoleLayout, device=None):
         from ..models.gpt import GPTModel
+        check_serving(cfg.sampler.infer_engine_configs[0])
         self.cfg, self.layout = cfg, layout
         self.rank = dist.get_rank()
         self.device = device or _dev()

@@ -11,7 +11,7 @@ from typing import List, Optional, Sequence
 import torch
 
 from ..core import parallel_state as ps
-from ..rollout.disaggregated import RemoteRollout, RoleLayout
+from ..rollout.disaggregated import RemoteRollout, RoleLayout, check_serving
 from ..rollout.engine import SamplingParams
 from .grpo_trainer import GrpoTrainer, response_mask
 
@@ -24,13 +24,12 @@ class DisaggGrpoTrainer(GrpoTrainer):
 
     def setup(self):
         cfg = self.cfg
-        self.policy.setup_model_and_get_optimizer()
         ie = cfg.sampler.infer_engine_configs[0]
+        check_serving(ie)
+        self.policy.setup_model_and_get_optimizer()
         self.policy.temperature = ie.temperature
         self.lora = bool(cfg.policy.lora.enabled)
         self.release_rollout_weights = False
-        if ie.fp4_weights:
-            raise NotImplementedError("fp4_weights: remote rollout engines serve the weights as they are sent")
         self.serve_fp8 = self.serve_fp4 = False
         self.engine = None
         self.sampling = SamplingParams(temperature=ie.temperature, top_k=ie.top_k, top_p=ie.top_p, min_p=ie.min_p, repetition_penalty=ie.repetition_penalty,

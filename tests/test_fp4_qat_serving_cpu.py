@@ -72,3 +72,17 @@ def test_adapters_and_block_fp8_are_refused_before_anything_is_built():
     for qat in (False, True):
         with pytest.raises(ValueError, match="LoRA"):
             trainer(qat=qat, lora=cfg.policy.lora)
+
+
+def test_engines_that_are_not_served_in_4_bits_say_so():
+    from types import SimpleNamespace
+    from gcore_b200.entry import lm_infer, train_lm_distill
+    from gcore_b200.rollout.disaggregated import SamplerServer
+    from gcore_b200.trainer.disagg_trainer import DisaggGrpoTrainer
+    cfg = make_cfg()
+    cfg.sampler.infer_engine_configs[0].fp4_weights = True
+    never = SimpleNamespace(cfg=cfg)   # whatever else they touch is missing
+    for call in (lambda: SamplerServer(cfg, None, None), lambda: DisaggGrpoTrainer.setup(never),
+                 lambda: train_lm_distill.off_policy_loop(never, [], 1, None), lambda: lm_infer.serve_checkpoint(cfg, {})):
+        with pytest.raises(NotImplementedError, match="fp4_weights"):
+            call()
