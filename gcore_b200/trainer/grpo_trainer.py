@@ -325,6 +325,7 @@ class GrpoTrainer:
             self.engine.update_weights(None)
         elif self.release_rollout_weights:
             self.engine.load_weights_from(self.policy.model, self.cfg.policy.sampler_client.update_weight_max_size_mb)
+            self._quantize_served_weights()   # the other two end in engine.update_weights, which does it
         else:
             from ..rollout.weight_sync import sync_weights
             sync_weights(self.policy, self.engine)
@@ -333,8 +334,6 @@ class GrpoTrainer:
             bad = verify(self.policy, self.engine)
             if bad:
                 raise RuntimeError(f"rollout weights differ from the trainer's after the hand-over: {bad[:6]}")
-        # the engine's dense projections are re-quantised from the weights just handed over
-        self._quantize_served_weights()
 
     def _quantize_served_weights(self):
         """Low-precision copies that the rollout engine serves: e4m3 with 128x128 scales, or 4 bits with one power of two per 32."""

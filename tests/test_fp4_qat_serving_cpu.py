@@ -86,3 +86,30 @@ def test_engines_that_are_not_served_in_4_bits_say_so():
                  lambda: train_lm_distill.off_policy_loop(never, [], 1, None), lambda: lm_infer.serve_checkpoint(cfg, {})):
         with pytest.raises(NotImplementedError, match="fp4_weights"):
             call()
+
+
+@pytest.mark.parametrize("policy", [dict(), dict(share_rollout_weights=False),
+                                    dict(share_rollout_weights=False, release_rollout_weights=True)])
+@pytest.mark.parametrize("mode", ["fp4", "fp8"])
+def test_a_hand_over_quantises_once(policy, mode, monkeypatch):
+    if mode == "fp4":
+        tr = trainer(**policy)
+    else:
+        tr = trainer_fp8(**policy)
+    name = f"quantize_weights_{mode}"
+    calls, quantise = [], getattr(tr.engine, name)
+    monkeypatch.setattr(tr.engine, name, lambda *a, **k: calls.append(a) or quantise(*a, **k))
+    tr.step(PROMPTS)
+    assert len(calls) == 1
+    lw = tr.engine.w.layers[0] if tr.engine.w is not None else None
+    assert lw is None or (lw.fp4 if mode == "fp4" else lw.fp8)
+
+
+def trainer_fp8(**policy):
+    cfg = make_cfg()
+    for k, v in policy.items():
+        setattr(cfg.policy, k, v)
+    cfg.sampler.infer_engine_configs[0].fp8_weights = True
+    mcfg = ModelConfig(arch="qwen2", num_layers=2, hidden_size=256, num_attention_heads=4, num_kv_heads=2, ffn_hidden_size=352,
+                       vocab_size=512, dtype="float32")
+    return GrpoTrainer(cfg, model_cfg=mcfg, reward_fn=reward_has_small_token).setup()
