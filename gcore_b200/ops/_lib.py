@@ -82,6 +82,8 @@ def kernels() -> ctypes.CDLL:
         cap = os.environ.get("GCORE_DECODE_SMEM_KB")   # shared-memory budget of decode GEMM CTAs (0 = full ring)
         if cap is not None and hasattr(lib, "gk_gemm_set_decode_smem_cap"):
             lib.gk_gemm_set_decode_smem_cap(int(cap) * 1024)
+        if os.environ.get("GCORE_PDL", "1") == "0" and hasattr(lib, "gk_set_overlap"):   # no launch overlaps the one in front
+            lib.gk_set_overlap(0)
         _KERNELS = lib
     return _KERNELS
 
@@ -205,6 +207,7 @@ def _declare_kernels(lib: ctypes.CDLL):
     d("gk_ep_pull", [P, P, P, P, P, I, I, I, I, L, P])
     d("gk_peer_copy_2d", [P, L, P, L, L, I, P])
     d("gk_set_pdl", [I], None)
+    d("gk_set_overlap", [I])
     d("gk_set_peer_wait_budget", [L], None)
     d("gk_peer_rows", [P, L, I, P, P])
     d("gk_allreduce_oneshot", [P, P, L, I, I, L, P, P, P, P])

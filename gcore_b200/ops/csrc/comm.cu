@@ -368,6 +368,12 @@ GK_EXPORT int gk_peer_rows(void* dst, long long n, int nseg, const unsigned long
 
 // 1: kernels of the decode chain are launched with programmatic stream serialization (see host_utils.h)
 GK_EXPORT void gk_set_pdl(int on) { gk::pdl_flag() = on; }
+// Whether kernels that wait by themselves may be set up while the kernel in front drains, in a decode chain or not; returns what held.
+GK_EXPORT int gk_set_overlap(int on) {
+  const int was = gk::overlap_flag();
+  gk::overlap_flag() = on != 0;
+  return was;
+}
 
 GK_EXPORT int gk_allreduce_ctas() { return AR_CTAS; }
 

@@ -986,7 +986,7 @@ inline int decode_launch(const void* codes, const void* xq, long long xq_rows, i
   attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   // Set up while the kernel in front drains.  What that kernel may have written is read behind the wait; the weight only where it
   // cannot have: behind the split of the same call, in a decode chain.
-  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].val.programmaticStreamSerializationAllowed = gk::overlap_flag();
   p.early = pl.src == SPLIT || gk::pdl_flag();
   cfg.attrs = attr;
   cfg.numAttrs = 2;
@@ -1013,7 +1013,7 @@ inline int prompt_launch(const void* codes, const void* xq, long long xq_rows, i
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;   // behind the kernel of the same call that prepares the tokens
+  attr[0].val.programmaticStreamSerializationAllowed = gk::overlap_flag();   // behind the kernel of the same call that prepares the tokens
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   return gk::launch_ex(cfg, fp4_prompt_kernel<TERMS>, tmW, tmX, p);

@@ -150,6 +150,11 @@ inline int& pdl_flag() {
   static int flag = 0;
   return flag;
 }
+// launch_waiting and the 4-bit products overlap outside of a decode chain too, unless gk_set_overlap(0).
+inline int& overlap_flag() {
+  static int flag = 1;
+  return flag;
+}
 template <typename... KArgs, typename... Args>
 inline void launch_k(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, Args... args) {
   if (!pdl_flag()) {
@@ -196,7 +201,7 @@ inline int launch_waiting(void (*kernel)(KArgs...), unsigned grid, unsigned bloc
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[0].val.programmaticStreamSerializationAllowed = overlap_flag();
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   return launch_ex(cfg, kernel, args...);
