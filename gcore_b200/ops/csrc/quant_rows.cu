@@ -331,10 +331,10 @@ GK_EXPORT int gk_norm_quant(const void* x, const void* res, const void* w, void*
   return as16 ? slots(N{}, Y{}) : slots(N{}, N{});
 }
 
-// act: in [T, 2 F] bf16 = [gate | up]; otherwise in [T, F].  q [T, F], scales as above; 16-byte aligned.
+// act: in [T, 2 F] bf16 = [gate | up]; otherwise in [T, F], with sc32 and without as16 only.  q [T, F], scales as above; 16-byte aligned.
 GK_EXPORT int gk_rows_quant(const void* in, void* q, void* scales, long long T, int F, int act, int sc32, int as16,
                             void* stream) {
-  if (T < 0 || F <= 0 || F % (sc32 ? 32 : 128)) return -1;
+  if (T < 0 || F <= 0 || F % (sc32 ? 32 : 128) || (!act && (!sc32 || as16))) return -1;
   if (!aligned16(in) || !aligned16(q)) return -2;
   if (T == 0) return 0;
   const int nv = F / 8;
@@ -350,7 +350,7 @@ GK_EXPORT int gk_rows_quant(const void* in, void* q, void* scales, long long T, 
   auto pick = [&](auto width, auto n) {
     using I = decltype(n);
     constexpr int U = decltype(width)::value;
-    if (!act) return sc32 ? go(rows_quant_kernel<false, true, false, U, I>, n) : go(rows_quant_kernel<false, false, false, U, I>, n);
+    if (!act) return go(rows_quant_kernel<false, true, false, U, I>, n);
     if (sc32) return as16 ? go(rows_quant_kernel<true, true, true, U, I>, n) : go(rows_quant_kernel<true, true, false, U, I>, n);
     return as16 ? go(rows_quant_kernel<true, false, true, U, I>, n) : go(rows_quant_kernel<true, false, false, U, I>, n);
   };
