@@ -345,6 +345,9 @@ class Fp4Weight:
         N, K = w.shape
         if K % 32:
             raise ValueError(f"Fp4Weight: {K} columns are not whole groups of 32")
+        if _lib.use_native(w) and not _lib.is_current(w):
+            with torch.cuda.device(w.device):
+                return cls.of(w)
         packed, e8, _ = quant_fp4_1x32(w.detach().contiguous())
         return cls(packed.view(N, K // 2), e8.view(N, K // 32))
 
