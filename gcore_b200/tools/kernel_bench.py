@@ -10,6 +10,9 @@ against the measured roofline denominators in ``MEASURED_PEAKS.json`` when prese
 ``python -m gcore_b200.tools.kernel_bench train_step --model qwen2.5-7b --layers 8 --tokens 8192 --seqlen 1280``
 ``python -m gcore_b200.tools.kernel_bench ce --tokens 8192 --vocab 152064 --k 3584 [--fused-only]``   vocabulary
                                                                  GEMM with softmax statistics vs the chunked form
+``python -m gcore_b200.tools.kernel_bench low_precision [--only norm]``   norms, activations and rows that end in e4m3 and
+                                                                 4-bit products under graph replay, beside the launches
+                                                                 they replace (norm + quantiser, bf16 or fp8 product)
 
 The single-shape sub-commands launch one kernel a few times, which also makes them the small cases profilers are
 pointed at.
@@ -618,6 +621,70 @@ def cmd_ce(argv=None):
 
 
 COMMANDS["ce"] = cmd_ce
+
+
+def cmd_low_precision(argv=None):
+    """The operators of low-precision serving inside a captured graph, inputs in turn from more than L2 holds, against what the
+    framework launches without them; in us a call."""
+    ap = argparse.ArgumentParser()
+    ap.add_argument("--only", default="", help="operators whose name starts so")
+    args = ap.parse_args(argv)
+    from gcore_b200.ops import _lib, fused, quant
+    from gcore_b200.ops.gemm import linear_forward
+
+    def rnd(*shape):
+        return torch.randn(*shape, device="cuda").bfloat16()
+
+    def report(name, make, new, old=None, other=""):
+        """``make()`` gives one set of inputs; ``new`` and ``old`` take it.  Not more of them than 300 MB hold."""
+        if not name.startswith(args.only):
+            return
+        first = make()
+        size = sum(t.numel() * t.element_size() for t in first if isinstance(t, torch.Tensor))
+        sets = [first] + [make() for _ in range(min(31, int(300e6 / max(size, 1))))]
+        n = max(8, len(sets))
+        row = {"name": name, "us": round(graph_time([lambda a=sets[i % len(sets)]: new(*a) for i in range(n)]), 2)}
+        if old is not None:
+            row[other] = round(graph_time([lambda a=sets[i % len(sets)]: old(*a) for i in range(n)]), 2)
+        print(json.dumps(row), flush=True)
+
+    with torch.no_grad():
+        for T, H, scales, residual in ((1, 3584, "fp32", True), (96, 7168, "e8m0", True), (96, 7168, "fp32", True),
+                                       (3001, 1536, "fp32", False), (16384, 4096, "e8m0", True), (16384, 4096, "fp32", True)):
+            quantise = quant.quant_act_1x32 if scales == "e8m0" else quant.quant_act_1x128
+            gain = rnd(H)
+            make = lambda: (rnd(T, H), rnd(T, H) if residual else None)   # noqa: E731
+            report(f"norm {T} x {H} {scales}", make, lambda x, r: fused.rmsnorm_fp8(x, gain, 1e-6, r, scales=scales))
+            report(f"norm {T} x {H} {scales} as_rounded", make,
+                   lambda x, r: fused.rmsnorm_fp8(x, gain, 1e-6, r, scales=scales, as_rounded=True),
+                   lambda x, r: quantise(fused.rmsnorm(x, gain, 1e-6, r)[0]), "norm_and_quantiser")
+        for T, F, scales in ((64, 18944, "fp32"), (64, 18944, "e8m0"), (8191, 14336, "e8m0"), (8191, 14336, "fp32")):
+            quantise = quant.quant_act_1x32 if scales == "e8m0" else quant.quant_act_1x128
+            make = lambda: (rnd(T, 2 * F),)   # noqa: E731
+            report(f"swiglu {T} x {F} {scales}", make, lambda x: fused.swiglu_fp8(x, scales=scales))
+            report(f"swiglu {T} x {F} {scales} as_rounded", make, lambda x: fused.swiglu_fp8(x, scales=scales, as_rounded=True),
+                   lambda x: quantise(fused.swiglu(x)), "activation_and_quantiser")
+        for T, K in ((64, 3584), (8192, 4096)):
+            report(f"rows {T} x {K} e8m0", lambda: (rnd(T, K),), lambda x: quant.quant_act_1x32(x),
+                   lambda x: quant.quant_act_1x128(x), "fp32_scales")
+        for T, N, K, bias in ((1, 37888, 3584, False), (13, 4608, 3584, True), (64, 3584, 18944, False), (3391, 6144, 4096, False)):
+            b = rnd(N) if bias else None
+
+            def make():
+                w = rnd(N, K) * 0.02
+                return rnd(T, K), quant.Fp4Weight.of(w), w
+            report(f"linear {T} x {N} x {K}", make, lambda x, W, w: quant.linear_fp4(x, W, b),
+                   lambda x, W, w: linear_forward(x, w, b), "bf16_weight")
+        for T, N, K in ((1, 28672, 4096), (96, 28672, 4096), (8192, 28672, 4096)):
+            def make():
+                x, w = rnd(T, K), rnd(N, K) * 0.02
+                return (*quant.quant_act_1x32(x), quant.Fp4Weight.of(w), *quant.quant_act_1x128(x), *quant.quant_weight_128x128(w))
+            report(f"gemm {T} x {N} x {K}", make, lambda q, s, W, *_: quant.gemm_fp4(q, s, W),
+                   lambda q, s, W, *fp8: quant.gemm_fp8_blockscaled(*fp8), "block_fp8_weight")
+    _lib.check_device_errors()
+
+
+COMMANDS["low_precision"] = cmd_low_precision
 
 
 def cmd_fused(argv=None):
