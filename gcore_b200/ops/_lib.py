@@ -120,12 +120,19 @@ def packed16(t: torch.Tensor) -> torch.Tensor:
     return t if t.is_contiguous() and t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
 
 
-def differentiated(*tensors) -> bool:
-    """Whether a derivative of one of the tensors (or None) is asked for: a gradient, or in forward mode a tangent."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        return True
+def has_tangent(*tensors) -> bool:
+    """Whether one of the tensors (or None) carries a tangent of forward-mode differentiation."""
     return forward_ad._current_level >= 0 and any(
         t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+
+
+def differentiated(*tensors) -> bool:
+    """Whether a derivative of one of the tensors (or None) is asked for: a gradient, or in forward mode a tangent."""
+    if torch.is_grad_enabled():
+        for t in tensors:   # a generator takes 0.3 us longer, a fiftieth of a call
+            if t is not None and t.requires_grad:
+                return True
+    return has_tangent(*tensors)
 
 
 def check(rc: int, what: str):

@@ -36,9 +36,9 @@ def test_product_carries_tangents_and_refuses_a_second_derivative(monkeypatch):
                         torch.nn.functional.linear(x2, w, bias).to(dtype))
     monkeypatch.setattr(quant, "_fp4_dgrad", lambda dy, weight: dy.detach().float() @ w)
     with fw.dual_level():
-        y = fw.unpack_dual(quant._LinearFp4.apply(fw.make_dual(x, t), W, fw.make_dual(b, 2 * b)))
+        y = fw.unpack_dual(quant._LinearFp4Tangent.apply(fw.make_dual(x, t), W, fw.make_dual(b, 2 * b)))
         assert torch.allclose(y.tangent, t @ w.t() + 2 * b, rtol=1e-5, atol=1e-5)
-        y = fw.unpack_dual(quant._LinearFp4.apply(x, W, fw.make_dual(b, 2 * b)))
+        y = fw.unpack_dual(quant._LinearFp4Tangent.apply(x, W, fw.make_dual(b, 2 * b)))
         assert y.tangent.shape == (3, 40) and torch.allclose(y.tangent.float(), (2 * b).expand(3, 40), rtol=2 ** -8)
     x.requires_grad_()
     g, = torch.autograd.grad(quant._LinearFp4.apply(x, W, None).square().sum(), x, create_graph=True)
