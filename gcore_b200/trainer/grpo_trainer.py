@@ -76,7 +76,7 @@ class GrpoTrainer:
     def setup(self):
         cfg = self.cfg
         ie = cfg.sampler.infer_engine_configs[0]
-        if ie.fp4_weights and cfg.policy.fp8:
+        if ie.fp4_weights and (ie.fp8_weights or cfg.policy.fp8):
             raise ValueError("the rollout engine serves its projections in 4 bits (fp4_weights) or in block fp8, not in both")
         if ie.fp4_weights and cfg.policy.lora.enabled:
             # the engine's weight is base + delta: rounded to 4 bits, most of a small delta goes and the rest is several times too large

@@ -68,6 +68,10 @@ def test_adapters_and_block_fp8_are_refused_before_anything_is_built():
     with pytest.raises(ValueError, match="not in both"):
         trainer(qat=False, fp8=True)
     cfg = make_cfg()
+    cfg.sampler.infer_engine_configs[0].fp4_weights = cfg.sampler.infer_engine_configs[0].fp8_weights = True
+    with pytest.raises(ValueError, match="not in both"):
+        GrpoTrainer(cfg, model_cfg=ModelConfig(num_layers=1, hidden_size=128, num_attention_heads=2, num_kv_heads=2, ffn_hidden_size=128,
+                                               vocab_size=512, dtype="float32"), reward_fn=reward_has_small_token).setup()
     cfg.policy.lora.rank = 8
     for qat in (False, True):
         with pytest.raises(ValueError, match="LoRA"):
