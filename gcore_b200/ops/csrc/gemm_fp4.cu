@@ -720,7 +720,7 @@ fp4_prompt_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant
         }
       }
       // A lane has a token's 128 features; through shared memory four lanes write 64 bytes of a token together, eight tokens an
-      // instruction (16 bytes of 32 tokens each: half-filled sectors, 787 us instead of 765 for 8192 x 28672 x 4096).
+      // instruction (16 bytes of 32 tokens each: half-filled sectors, 3 % longer for 8192 x 28672 x 4096).
       uint8_t* patch = patches + (warp - 2) * C::PATCH;
       if ((p.ldy & 7) == 0 && col0 + 128 <= p.N) {
         const int width = p.out_fp32 ? 16 : 32;   // features of a patch
@@ -894,7 +894,8 @@ struct Fp4Plan {
 // rate; all together get 9.5 KB a ns out of L2.  A round of CTAs costs 2 and Tc / 50 for each CTA of an SM, a launch 2, the
 // exchange in a cluster 2 + Tc / 33 and 1 more for eight CTAs, of which fewer fit into a GPC.  Chosen against the others that were
 // run, ks = 1 / 2 / 4 / 8: 1 x 4608 x 3584 12.0 / 9.5 / [9.0] / 9.8, 64 x 4608 x 3584 [14.1] / 14.6 / 21.0 / 26.1, 64 x 3584 x 18944
-// 45.7 / 31.8 / [20.6] / 27.6, 16 x 3584 x 18944 - / 25.4 / [16.7] / 15.2, 96 x 28672 x 4096 (e4m3) [23.1] / 67 / 89 / 154; one or two
+// 45.7 / 31.8 / [20.6] / 27.6, 16 x 3584 x 18944 - / 25.4 / [16.7] / 15.2 (a second round
+// of few CTAs counts as a whole one: 26 by the model), 96 x 28672 x 4096 (e4m3) [23.1] / 67 / 89 / 154; one or two
 // CTAs an SM: 1 x 37888 x 3584 22.6 / [16.0], 64 x 4608 x 3584 [14.1] / 16.3.
 inline Fp4Plan decode_plan(int T, int Tc, int terms, int N, int kb) {
   Fp4Plan p = {}, best = {};

@@ -358,7 +358,9 @@ def rmsnorm_fp8(x: torch.Tensor, w: torch.Tensor, eps: float = 1e-6, residual: t
     ``residual`` the third value is ``x``).  ``scales="fp32"``: ``s`` has one 32-bit scale per 128 values, what
     ``quant.gemm_fp8_blockscaled`` reads; ``"e8m0"``: one power of two per 32 values (``torch.float8_e8m0fnu``), what
     ``quant.gemm_fp4`` reads.  The norm is rounded once, to e4m3; with ``as_rounded`` it is rounded to ``x``'s type first, so that
-    ``q`` and ``s`` are those of ``quant_act_1x128(rmsnorm(...)[0])`` bit for bit.  Inference only."""
+    ``q`` and ``s`` are those of ``quant_act_1x128(rmsnorm(...)[0])`` bit for bit (``e8m0``: ``quant_act_1x32``; rows of more than 8192
+    values, whose ``rmsnorm`` adds up in another order, up to that).  On a GPU bf16 rows of up to 16384 values are one kernel; other
+    types and widths are computed in 32 bits by PyTorch.  Inference only."""
     H = x.shape[-1]
     if w.dim() != 1 or w.shape[0] != H or (residual is not None and residual.shape != x.shape):
         raise ValueError(f"rmsnorm_fp8: x {tuple(x.shape)}, gain {tuple(w.shape)}"
@@ -391,7 +393,7 @@ def rmsnorm_fp8(x: torch.Tensor, w: torch.Tensor, eps: float = 1e-6, residual: t
 
 def swiglu_fp8(x: torch.Tensor, scales: str = "fp32", as_rounded: bool = False):
     """``swiglu`` whose result is quantised in the same pass: ``(q, s)`` with ``q`` e4m3 ``[..., F]`` for ``x`` ``[..., 2 F]``;
-    ``scales`` and ``as_rounded`` as in ``rmsnorm_fp8``.  Inference only."""
+    ``scales`` and ``as_rounded`` as in ``rmsnorm_fp8``, types other than bf16 too.  Inference only."""
     if x.shape[-1] % 2:
         raise ValueError(f"swiglu_fp8: x {tuple(x.shape)} is not [gate | up]")
     F = x.shape[-1] // 2

@@ -469,7 +469,8 @@ class _LinearFp4Tangent(_LinearFp4):
 
 def linear_fp4(x: torch.Tensor, weight: Fp4Weight, bias: torch.Tensor | None = None) -> torch.Tensor:
     """``y = x W^T (+ bias)`` for a frozen 4-bit weight and 16-bit activations, ``x`` [..., K] -> [..., N] in ``x``'s type: the
-    product that a model trained with ``fp4_qat`` computes.  Differentiable once in ``x`` and ``bias``, in reverse and forward mode."""
+    product that a model trained with ``fp4_qat`` computes.  Differentiable once in ``x`` and ``bias``, in reverse and forward mode.
+    On a GPU bf16 activations run on the kernels; others are multiplied in 32 bits by PyTorch with the weight's values, made anew."""
     _check_fp4("linear_fp4", x, weight, bias)
     N, K = weight.shape
     if not (_lib.use_native(x) and x.dtype == torch.bfloat16):
