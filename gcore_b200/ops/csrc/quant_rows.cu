@@ -210,8 +210,8 @@ __global__ void __launch_bounds__(256) norm_quant_kernel(const Row8* __restrict_
 
 // A unit of the activation whose gates may be far below zero: e^-gate or its reciprocal leaves the 32-bit range there, and a large
 // partner brings the product back.  With h = e^(-|gate| / 2): gate / (1 + h^2), times h^2 where the gate is negative, half of it in
-// front of the partner and half behind.  (us, for all units / in a second pass of
-// the warps that need it / not at all: 8191 x 14336 99.7 / 90.6 / 90.2.)
+// front of the partner and half behind.  (For all units it takes 99.7 us instead of 90.2, 8191 x 14336: a second pass of
+// rows_quant_kernel does it where it is needed.)
 template <bool SC32>
 __device__ __noinline__ void far_gates(const Row8* __restrict__ in, long long u, bool live, int nv, uint2* __restrict__ q,
                                        void* __restrict__ scales) {
@@ -238,8 +238,9 @@ __global__ void __launch_bounds__(256) rows_quant_kernel(const Row8* __restrict_
   pdl_launch_dependents();
   pdl_wait();
   const long long step = static_cast<long long>(gridDim.x) * (256 * U);
-  uint32_t far = 0;   // the largest bit patterns of gates: those furthest below zero
+  uint32_t redo = 0, turn = 1;   // iterations with gates far below zero; the last bit stands for all from the 32nd on
   for (long long u0 = blockIdx.x * (256ll * U); u0 < units; u0 += step) {
+    uint32_t far = 0;   // the largest bit patterns of gates: those furthest below zero
     Row8 a[U], b[U];
     // one division for all units of an iteration where they span two rows at most
     const bool few = ACT && nv >= 256 * U;
@@ -285,16 +286,26 @@ __global__ void __launch_bounds__(256) rows_quant_kernel(const Row8* __restrict_
       }
       quantise<SC32, AS16, false>(f, 1.f, u < units, u, q, scales);
     }
+    if (ACT && !AS16) {
+      if (max(far >> 16, far & 0xffffu) > 0xc2a0u) redo |= turn;
+      if (turn < 0x80000000u) turn <<= 1;
+    }
   }
-  // Below a gate of -87 that is zero, as in swiglu.  Where nothing is rounded in between, a warp that has seen a gate below -80 (0xc2a0)
-  // does its units over.
-  if (ACT && !AS16 && __any_sync(0xffffffffu, max(far >> 16, far & 0xffffu) > 0xc2a0u)) {
-    for (long long u0 = blockIdx.x * (256ll * U); u0 < units; u0 += step) {
+  // Below a gate of -87 that is zero, as in swiglu.  Where nothing is rounded in between, a warp does the units of the iterations over
+  // in which it has a gate below -80 (0xc2a0).  us, 8191 x 14336, without such gates / with a channel of them / with a token in 100 /
+  // nothing else: this 91.0 / 99 / 93 / 208, the whole share of a warp over 90.5 / 133 / 102 / 202, no second pass 90.1.
+  if (ACT && !AS16) {
+    redo = __reduce_or_sync(0xffffffffu, redo);
+    turn = 1;
+    for (long long u0 = blockIdx.x * (256ll * U); redo && u0 < units; u0 += step) {
+      if (redo & turn) {
 #pragma unroll 1
-      for (int k = 0; k < U; ++k) {
-        const long long u = u0 + k * 256 + static_cast<int>(threadIdx.x);
-        far_gates<SC32>(in, u, u < units, nv, q, scales);
+        for (int k = 0; k < U; ++k) {
+          const long long u = u0 + k * 256 + static_cast<int>(threadIdx.x);
+          far_gates<SC32>(in, u, u < units, nv, q, scales);
+        }
       }
+      if (turn < 0x80000000u) turn <<= 1;
     }
   }
 }

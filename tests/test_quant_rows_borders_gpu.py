@@ -86,6 +86,24 @@ def test_a_few_far_gates_in_a_large_batch(scales):
     assert same > 0.999
 
 
+def test_far_gates_late_in_a_share():
+    """More than 32 iterations a thread: those beyond share a bit of what is to be done over."""
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    F = 16384
+    T = 36 * sms * 32 * 512 // (F // 8)
+    x = torch.randn(2, 2 * F, generator=torch.Generator(device="cuda").manual_seed(2), device="cuda").bfloat16().repeat(T // 2, 1)
+    T = x.shape[0]
+    rows = [0, 3, T // 36 * 30, T // 36 * 34 + 1, T - 1]
+    x[rows, :F] = (-84 - 6 * torch.rand(5, F, generator=torch.Generator(device="cuda").manual_seed(3), device="cuda")).bfloat16()
+    x[rows, F:] *= 1e30
+    q, s = fused.swiglu_fp8(x, scales="e8m0")
+    some = rows + [1, 2, T // 2, T - 2]
+    g, u = x[some].double().chunk(2, -1)
+    check(q[some], s[some], g * torch.sigmoid(g) * u, "e8m0", 2 ** -16)
+    plain = [i for i in range(100, T - 100, 2) if i not in rows]   # copies of row 0 as it was
+    assert (q.view(torch.uint8)[plain] == q.view(torch.uint8)[plain[0]]).all()
+
+
 @pytest.mark.parametrize("T,H", [(1, 3584), (37, 4096), (200, 96), (3, 8192)])
 def test_rounded_forms_with_powers_of_two_are_the_chains_bit_for_bit(T, H):
     x, r, w = rand(T, H, seed=1), rand(T, H, seed=2, scale=3), 1 + rand(H, seed=3, scale=0.2)
